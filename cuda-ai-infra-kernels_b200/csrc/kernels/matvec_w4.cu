@@ -1,0 +1,241 @@
+// Matrix-vector product with 4-bit weights and group scales, for 1 to 16 rows of x.
+//
+// Bound by HBM: every weight byte is read once, 2 * rows products per weight. The arithmetic must
+// therefore cost a handful of instructions per eight weights, and goes through the warp-level matrix
+// instruction m16n8k16 with the weights as its 16-row operand and the rows of x as its columns: the
+// 5th-generation tensor cores would want 128 weight rows per tile in shared memory, a detour for
+// bytes that are used once; here they go from global memory to registers to the multiply.
+//
+// A warp owns 16 rows of weights and a range of K. The sum over k does not care about its order, so
+// each of the four threads that share a row takes its own run of consecutive weights (kBytes bytes
+// per load) instead of the interleaved pairs that the instruction nominally wants, and loads the
+// same run of x. Nibbles i and i + 4 of a 32-bit word become one pair of 16-bit values: the bits of
+// a code c placed into the mantissa of 1024 (FP16) or 128 (BF16) give 1024 + c or 128 + c exactly, and
+// subtracting 1024 + zero or 128 + zero leaves c - zero, exact. Each step of K lies inside one group:
+// its FP32 product is multiplied by the group's scale when it is added to the running sum.
+//
+// FP32 x is written as the sum of three BF16 numbers (8 + 8 + 8 bits, by truncation: exact), which take
+// three columns of the instruction and are added up at the end, so that products and sums are as
+// accurate as FP32 arithmetic.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "host_common.h"
+#include "ptx_sm100.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kMaxRows = 16;
+
+struct W4Args {
+  b200_matvec_w4_problem q;
+};
+
+template <typename T> struct Pair;
+template <> struct Pair<__half> {
+  static constexpr uint32_t kBase = 0x64006400u;   // 1024, 1024
+  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
+    const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+template <> struct Pair<__nv_bfloat16> {
+  static constexpr uint32_t kBase = 0x43004300u;   // 128, 128
+  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+template <> struct Pair<float> : Pair<__nv_bfloat16> {};   // FP32 x travels as three BF16 columns
+
+template <int kBytes> struct Packed;
+template <> struct Packed<16> {
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const uint8_t* p) {
+    const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  }
+};
+template <> struct Packed<8> {
+  uint32_t w[2];
+  __device__ __forceinline__ void load(const uint8_t* p) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    w[0] = v.x, w[1] = v.y;
+  }
+};
+template <> struct Packed<4> {
+  uint32_t w[1];
+  __device__ __forceinline__ void load(const uint8_t* p) { w[0] = __ldg(reinterpret_cast<const uint32_t*>(p)); }
+};
+
+// Eight consecutive x of one column as four pairs (x0,x4), (x1,x5), (x2,x6), (x3,x7).
+template <typename T>
+__device__ __forceinline__ void load_pairs(uint32_t (&out)[4], const T* p, int) {
+  const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));   // (x0,x1) (x2,x3) (x4,x5) (x6,x7)
+  out[0] = __byte_perm(v.x, v.z, 0x5410), out[1] = __byte_perm(v.x, v.z, 0x7632);
+  out[2] = __byte_perm(v.y, v.w, 0x5410), out[3] = __byte_perm(v.y, v.w, 0x7632);
+}
+// Term `part` of a finite FP32 number as a sum of three BF16 ones, in the upper half of the result.
+__device__ __forceinline__ uint32_t bf16_term(float x, int part) {
+  const uint32_t hi = __float_as_uint(x) & 0xffff0000u;
+  if (part == 0) return hi;
+  // What an infinity or a NaN leaves is nothing: the first term carries it alone.
+  const float r1 = (hi & 0x7f800000u) == 0x7f800000u ? 0.f : x - __uint_as_float(hi);
+  const uint32_t mid = __float_as_uint(r1) & 0xffff0000u;
+  if (part == 1) return mid;
+  return __float_as_uint(r1 - __uint_as_float(mid));
+}
+template <>
+__device__ __forceinline__ void load_pairs<float>(uint32_t (&out)[4], const float* p, int part) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  out[0] = __byte_perm(bf16_term(a.x, part), bf16_term(b.x, part), 0x7632);
+  out[1] = __byte_perm(bf16_term(a.y, part), bf16_term(b.y, part), 0x7632);
+  out[2] = __byte_perm(bf16_term(a.z, part), bf16_term(b.z, part), 0x7632);
+  out[3] = __byte_perm(bf16_term(a.w, part), bf16_term(b.w, part), 0x7632);
+}
+
+__device__ __forceinline__ float scale_at(const void* scales, int dtype, int64_t at) {
+  if (dtype == B200_FP32) return __ldg(static_cast<const float*>(scales) + at);
+  if (dtype == B200_FP16) return __half2float(__ldg(static_cast<const __half*>(scales) + at));
+  return __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(scales) + at));
+}
+__device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_out(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void store_out(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// kTiles groups of eight columns; kBytes weight bytes per thread, row and step (a step is 8 * kBytes
+// values of K: it has to lie inside a group).
+template <typename T, int kTiles, int kBytes>
+__global__ void __launch_bounds__(kWarps * 32) matvec_w4_kernel(const W4Args a) {
+  constexpr int kParts = sizeof(T) == 4 ? 3 : 1;   // columns per row of x
+  constexpr int kStep = 8 * kBytes;
+  __shared__ float sums[kWarps][16][8 * kTiles + 1];
+  const b200_matvec_w4_problem& q = a.q;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int quad = lane >> 2, t = lane & 3;
+  const int row0 = blockIdx.x * 16;
+  const int groups = q.k / q.group;
+  // Rows behind the last are read as the last one and not stored.
+  const int64_t r[2] = {min(row0 + quad, q.n - 1), min(row0 + quad + 8, q.n - 1)};
+  const int steps = q.k / kStep;
+  const int begin = static_cast<int>(static_cast<int64_t>(steps) * warp / kWarps), end = static_cast<int>(static_cast<int64_t>(steps) * (warp + 1) / kWarps);
+  const uint8_t* w0 = q.qweight + r[0] * (q.k / 2) + t * kBytes;
+  const uint8_t* w1 = q.qweight + r[1] * (q.k / 2) + t * kBytes;
+
+  float total[kTiles][4] = {};
+#pragma unroll 4
+  for (int s = begin; s < end; ++s) {
+    Packed<kBytes> p0, p1;
+    p0.load(w0 + static_cast<int64_t>(s) * (kStep / 2));
+    p1.load(w1 + static_cast<int64_t>(s) * (kStep / 2));
+    const int group = s * kStep / q.group;
+    const int64_t at0 = r[0] * groups + group, at1 = r[1] * groups + group;
+    const float scale0 = scale_at(q.scales, q.scale_dtype, at0), scale1 = scale_at(q.scales, q.scale_dtype, at1);
+    const uint32_t z0 = q.zeros == nullptr ? 8u : __ldg(q.zeros + at0) & 15u, z1 = q.zeros == nullptr ? 8u : __ldg(q.zeros + at1) & 15u;
+    const uint32_t base0 = Pair<T>::kBase | z0 | z0 << 16, base1 = Pair<T>::kBase | z1 | z1 << 16;
+    float acc[kTiles][4] = {};
+#pragma unroll
+    for (int i = 0; i < kBytes / 4; ++i) {
+      uint32_t m0[4], m1[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        m0[j] = Pair<T>::sub((p0.w[i] >> (4 * j) & 0x000f000fu) | Pair<T>::kBase, base0);
+        m1[j] = Pair<T>::sub((p1.w[i] >> (4 * j) & 0x000f000fu) | Pair<T>::kBase, base1);
+      }
+      const int64_t k = static_cast<int64_t>(s) * kStep + t * 2 * kBytes + i * 8;
+#pragma unroll
+      for (int c = 0; c < kTiles; ++c) {
+        const int column = c * 8 + quad;
+        uint32_t x[4] = {0, 0, 0, 0};
+        if (column < q.rows * kParts) load_pairs<T>(x, static_cast<const T*>(q.x) + static_cast<int64_t>(column / kParts) * q.k + k, column % kParts);
+        const uint32_t first[4] = {m0[0], m1[0], m0[1], m1[1]}, second[4] = {m0[2], m1[2], m0[3], m1[3]};
+        Pair<T>::mma(acc[c], first, x[0], x[1]);
+        Pair<T>::mma(acc[c], second, x[2], x[3]);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < kTiles; ++c) {
+      total[c][0] += scale0 * acc[c][0], total[c][1] += scale0 * acc[c][1];
+      total[c][2] += scale1 * acc[c][2], total[c][3] += scale1 * acc[c][3];
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < kTiles; ++c) {
+    sums[warp][quad][c * 8 + 2 * t] = total[c][0], sums[warp][quad][c * 8 + 2 * t + 1] = total[c][1];
+    sums[warp][quad + 8][c * 8 + 2 * t] = total[c][2], sums[warp][quad + 8][c * 8 + 2 * t + 1] = total[c][3];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * q.rows; i += kWarps * 32) {
+    const int n = i % 16, m = i / 16;
+    if (row0 + n >= q.n) continue;
+    float sum = 0.f;
+    for (int w = 0; w < kWarps; ++w)
+#pragma unroll
+      for (int part = 0; part < kParts; ++part) sum += sums[w][n][m * kParts + part];
+    store_out(static_cast<T*>(q.y) + static_cast<int64_t>(m) * q.n + row0 + n, sum);
+  }
+}
+
+template <typename T, int kTiles, int kBytes>
+int launch(const b200_matvec_w4_problem& q, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(q.n) + 15) / 16));
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.stream = s;
+  const GemmLaunchAttributes attrs = gemm_launch_attributes(1);
+  cfg.attrs = const_cast<cudaLaunchAttribute*>(attrs.list);
+  cfg.numAttrs = attrs.count;
+  if (cudaLaunchKernelEx(&cfg, matvec_w4_kernel<T, kTiles, kBytes>, W4Args{q}) != cudaSuccess) return launch_failed();
+  return launch_status();
+}
+
+template <typename T, int kTiles>
+int launch_bytes(const b200_matvec_w4_problem& q, cudaStream_t s) {
+  if (q.group % 128 == 0) return launch<T, kTiles, 16>(q, s);
+  if (q.group % 64 == 0) return launch<T, kTiles, 8>(q, s);
+  return launch<T, kTiles, 4>(q, s);
+}
+
+template <typename T>
+int launch_tiles(const b200_matvec_w4_problem& q, cudaStream_t s) {
+  const int columns = q.rows * (sizeof(T) == 4 ? 3 : 1);
+  if (columns <= 8) return launch_bytes<T, 1>(q, s);
+  if (columns <= 16) return launch_bytes<T, 2>(q, s);
+  if constexpr (sizeof(T) == 4) return columns <= 24 ? launch_bytes<T, 3>(q, s) : launch_bytes<T, 6>(q, s);
+  return B200_ERR_INTERNAL;
+}
+
+}  // namespace
+}  // namespace b200
+
+extern "C" int b200_matvec_w4(const b200_matvec_w4_problem* problem, b200_stream_t stream) {
+  if (problem == nullptr) return B200_ERR_INVALID_ARGUMENT;
+  const b200_matvec_w4_problem& q = *problem;
+  if (q.dtype < B200_FP32 || q.dtype > B200_BF16 || (q.scale_dtype != q.dtype && q.scale_dtype != B200_FP32)) return B200_ERR_INVALID_ARGUMENT;
+  if (q.rows < 0 || q.n < 0 || q.k <= 0 || q.group <= 0) return B200_ERR_INVALID_ARGUMENT;
+  if (q.rows > b200::kMaxRows) return B200_ERR_NOT_SUPPORTED;
+  if (q.group % 32 != 0 || q.k % q.group != 0) return B200_ERR_INVALID_PROBLEM;
+  if (q.rows == 0 || q.n == 0) return B200_OK;
+  if (q.x == nullptr || q.qweight == nullptr || q.scales == nullptr || q.y == nullptr) return B200_ERR_INVALID_ARGUMENT;
+  if (reinterpret_cast<uintptr_t>(q.x) % 16 != 0 || reinterpret_cast<uintptr_t>(q.qweight) % 16 != 0) return B200_ERR_MISALIGNED_OPERAND;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (q.dtype) {
+    case B200_FP32: return b200::launch_tiles<float>(q, s);
+    case B200_FP16: return b200::launch_tiles<__half>(q, s);
+    default: return b200::launch_tiles<__nv_bfloat16>(q, s);
+  }
+}

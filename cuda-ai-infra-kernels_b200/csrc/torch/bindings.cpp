@@ -1,7 +1,7 @@
 // pybind11 module `cuda_ai_kernels._C`: the 23 functions of the reference
 // module (csrc/bindings.cpp:10-45) with identical names, positional order,
-// keyword names and defaults, plus one introspection helper and the two fused all-gather entries of the
-// multi-GPU path.
+// keyword names and defaults, plus one introspection helper, the two fused all-gather entries of the
+// multi-GPU path and the four serving operators.
 #include <torch/extension.h>
 
 #include "ops.h"
@@ -42,4 +42,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("epilogue") = "linear", py::arg("kernel") = "auto", py::arg("out"), py::arg("peer_ptrs"));
   m.def("adaptive_gemm_last_kernel", &adaptive_gemm_last_kernel,
         "Registry name chosen by this thread's last adaptive_gemm call");
+  m.def("attention_prompt", &attention_prompt, "Attention over packed prompts", py::arg("q"), py::arg("k"), py::arg("v"),
+        py::arg("cu_seqlens_q"), py::arg("cu_seqlens_k") = py::none(), py::arg("causal") = true, py::arg("scale") = py::none());
+  m.def("attention_shared_prefix", &attention_shared_prefix, "One decoding step of a batch that shares a prefix", py::arg("q"),
+        py::arg("k_prefix"), py::arg("v_prefix"), py::arg("k_cache"), py::arg("v_cache"), py::arg("lengths"),
+        py::arg("scale") = py::none());
+  m.def("matvec_w4", &matvec_w4, "Product of 1 to 16 rows with 4-bit weights and group scales", py::arg("x"), py::arg("qweight"),
+        py::arg("scales"), py::arg("zeros") = py::none());
+  m.def("process_logits", &process_logits, "Penalties, sparse bias and grammar mask on logits", py::arg("logits"),
+        py::arg("prompt_tokens") = py::none(), py::arg("output_tokens") = py::none(), py::arg("repetition_penalty") = py::none(),
+        py::arg("frequency_penalty") = py::none(), py::arg("presence_penalty") = py::none(), py::arg("bias_ids") = py::none(),
+        py::arg("bias_values") = py::none(), py::arg("allowed") = py::none());
 }

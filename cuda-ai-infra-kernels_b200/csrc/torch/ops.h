@@ -51,3 +51,17 @@ torch::Tensor rmsnorm_cache_x(torch::Tensor x, torch::Tensor weight, double eps)
 torch::Tensor softmax_naive(torch::Tensor x);
 torch::Tensor rope_forward(torch::Tensor x, torch::Tensor cos, torch::Tensor sin);
 torch::Tensor attention_decode_forward(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache);
+
+// Serving operators (not part of the reference module).
+torch::Tensor attention_prompt(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& cu_seqlens_q,
+                               const c10::optional<at::Tensor>& cu_seqlens_k, bool causal, c10::optional<double> scale);
+torch::Tensor attention_shared_prefix(const torch::Tensor& q, const torch::Tensor& k_prefix, const torch::Tensor& v_prefix,
+                                      const torch::Tensor& k_cache, const torch::Tensor& v_cache, const torch::Tensor& lengths,
+                                      c10::optional<double> scale);
+torch::Tensor matvec_w4(const torch::Tensor& x, const torch::Tensor& qweight, const torch::Tensor& scales,
+                        const c10::optional<at::Tensor>& zeros);
+torch::Tensor process_logits(const torch::Tensor& logits, const c10::optional<at::Tensor>& prompt_tokens,
+                             const c10::optional<at::Tensor>& output_tokens, const c10::optional<at::Tensor>& repetition_penalty,
+                             const c10::optional<at::Tensor>& frequency_penalty, const c10::optional<at::Tensor>& presence_penalty,
+                             const c10::optional<at::Tensor>& bias_ids, const c10::optional<at::Tensor>& bias_values,
+                             const c10::optional<at::Tensor>& allowed);

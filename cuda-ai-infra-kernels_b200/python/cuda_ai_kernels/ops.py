@@ -114,3 +114,98 @@ def adaptive_gemm(
         epilogue,
         kernel,
     )
+
+
+# ---------------------------------------------------------------- serving operators
+# What one serving step of a decoder needs next to the products and row operators above. The
+# reference has none of them. They compute no gradient (inputs that require one are refused outside
+# ``torch.no_grad()``), run on the inputs' device and its current stream, read lengths and offsets on
+# the device only, and may be captured in CUDA graphs.
+
+
+def attention_prompt(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    cu_seqlens_k: Optional[torch.Tensor] = None,
+    causal: bool = True,
+    scale: Optional[float] = None,
+) -> torch.Tensor:
+    """Attention over packed prompts; ``[rows, heads, dim]`` in and out.
+
+    Sequence ``s`` owns the rows ``cu_seqlens_q[s]:cu_seqlens_q[s + 1]`` of ``q`` and
+    ``cu_seqlens_k[s]:cu_seqlens_k[s + 1]`` of ``k`` and ``v`` (int32 offsets; those of
+    ``q`` serve for both when ``cu_seqlens_k`` is left out). Query head ``h`` reads key
+    head ``h // (heads / kv_heads)``. Of ``m`` keys, query ``i`` of ``n`` sees the first
+    ``m - n + i + 1`` when ``causal`` (a chunk of a prompt, or a single token, at the end
+    of its cached keys), else all. ``scale`` defaults to ``dim ** -0.5``.
+
+    Rows that see no key, and rows behind the last sequence, are zero. Types: float32
+    (FP32 arithmetic), float16, bfloat16 (tensor cores, FP32 sums). ``dim`` is a multiple
+    of 8 up to 128. Strided views are taken as they are where their rows sit on 16-byte
+    granules, and copied otherwise. Keys and values outside a sequence may hold anything;
+    inside one, ``v`` must be finite.
+    """
+    return _C.attention_prompt(q, k, v, cu_seqlens_q, cu_seqlens_k, causal, scale)
+
+
+def attention_shared_prefix(
+    q: torch.Tensor,
+    k_prefix: torch.Tensor,
+    v_prefix: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    lengths: torch.Tensor,
+    scale: Optional[float] = None,
+) -> torch.Tensor:
+    """One decoding step of a batch whose requests share a prefix.
+
+    ``q`` is ``[batch, heads, dim]``, one token per request. Request ``b`` sees all of
+    ``k_prefix`` / ``v_prefix`` ``[prefix, kv_heads, dim]``, which are read once for the
+    whole batch, and the first ``lengths[b]`` rows of ``k_cache[b]`` / ``v_cache[b]``
+    (``[batch, room, kv_heads, dim]``); the rows behind may hold anything. Types, head
+    dimensions, strides and ``scale`` as for :func:`attention_prompt`. A request that
+    sees no key gets zeros.
+    """
+    return _C.attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, lengths, scale)
+
+
+def matvec_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x @ W.T`` for 1 to 16 rows ``x`` ``[rows, k]`` and 4-bit weights.
+
+    ``W[n, j] = (code[n, j] - zeros[n, j // group]) * scales[n, j // group]``, with the
+    codes packed two to a byte in ``qweight`` (uint8 ``[n, k / 2]``, the even ``j`` in the
+    low half), ``scales`` ``[n, k / group]`` in float32 or ``x``'s type, and ``zeros`` uint8
+    of the same shape (0 .. 15; 8 throughout when left out). The group size is
+    ``k / scales.shape[1]`` and a multiple of 32. ``x`` is float32, float16 or bfloat16;
+    products are exact in the codes, sums are FP32.
+    """
+    return _C.matvec_w4(x, qweight, scales, zeros)
+
+
+def process_logits(
+    logits: torch.Tensor,
+    prompt_tokens: Optional[torch.Tensor] = None,
+    output_tokens: Optional[torch.Tensor] = None,
+    repetition_penalty: Optional[torch.Tensor] = None,
+    frequency_penalty: Optional[torch.Tensor] = None,
+    presence_penalty: Optional[torch.Tensor] = None,
+    bias_ids: Optional[torch.Tensor] = None,
+    bias_values: Optional[torch.Tensor] = None,
+    allowed: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Logits ``[rows, vocab]`` made ready for :func:`softmax`, as a new tensor.
+
+    In this order, for row ``r`` and token ``t``: a token in the row's ``prompt_tokens`` or
+    ``output_tokens`` is divided by ``repetition_penalty[r]`` where positive and multiplied
+    by it otherwise; ``frequency_penalty[r]`` is subtracted once per occurrence in
+    ``output_tokens`` and ``presence_penalty[r]`` once if there is any; each entry ``i``
+    with ``bias_ids[r, i] == t`` adds ``bias_values[r, i]``; a token whose bit
+    ``t % 32`` of word ``t // 32`` of ``allowed`` is clear becomes minus infinity, whatever
+    it was. Token and bias ids are int32 ``[rows, length]``, and ids outside the vocabulary
+    are padding; penalties and bias values are float32; ``allowed`` is int32
+    ``[rows or 1, (vocab + 31) // 32]``. Arithmetic is FP32, rounded once.
+    """
+    return _C.process_logits(logits, prompt_tokens, output_tokens, repetition_penalty, frequency_penalty, presence_penalty,
+                             bias_ids, bias_values, allowed)

@@ -4,7 +4,8 @@
  * Hand-written sm_100a kernels for the operator set of the
  * "cuda-ai-infra-kernels" project: the FP32 SIMT GEMM ladder, the TF32
  * tensor-core GEMM with fused LinearCombination / ReLU epilogues and its
- * compatibility registry, and the RMSNorm / softmax row operators.
+ * compatibility registry, the RMSNorm / softmax row operators, and the operators of a
+ * serving step (attention, 4-bit matrix-vector product, logits).
  *
  * Conventions shared by every entry point
  *   - plain pointers and sizes only; nothing in this header depends on PyTorch
@@ -83,7 +84,8 @@ enum {
   B200_WAIT_UMMA_STORE = 1 << 6,
   B200_WAIT_SELFTEST = 1 << 7,      /* b200_selftest_wait_gives_up */
   B200_WAIT_PEER_BARRIER = 1 << 8,  /* b200_peer_barrier: a peer never signalled the step */
-  B200_WAIT_ROW_STAGED = 1 << 9     /* row operators: a row staged by the copy engine never arrived */
+  B200_WAIT_ROW_STAGED = 1 << 9,    /* row operators: a row staged by the copy engine never arrived */
+  B200_WAIT_ATTENTION = 1 << 11     /* attention: a pipeline stage never arrived (bit 10: debug build's index checks) */
 };
 
 /*
@@ -333,6 +335,130 @@ typedef enum b200_softmax_impl {
 /* y[r,:] = softmax(x[r,:]) over the last dimension, FP32, row-major [rows, cols]. */
 int b200_softmax(int impl, const float* x, float* y,
                  int64_t rows, int64_t cols, b200_stream_t stream);
+
+/* -------------------------------------------------------- serving operators */
+
+/*
+ * Operators of one serving step of a decoder, next to the matrix products and the
+ * row operators above. The reference declares attention (csrc/attention/
+ * attention_decode.cu:4-9) without implementing it and has no counterpart of the
+ * other three. They compute no gradients.
+ */
+typedef enum b200_dtype { B200_FP32 = 0, B200_FP16 = 1, B200_BF16 = 2 } b200_dtype;
+
+/* Strides of a [rows][heads][dim] array in elements; the last dimension is dense. */
+typedef struct b200_rows_view {
+  const void* data;
+  int64_t row_stride, head_stride;
+} b200_rows_view;
+
+/*
+ * Attention over packed prompts. Sequence s owns the query rows
+ * [cu_q[s], cu_q[s+1]) and the key rows [cu_k[s], cu_k[s+1]); query head h reads
+ * key head h / (heads / kv_heads). With n queries and m keys, and `causal` set,
+ * query i sees the keys j <= i + m - n (the last query sees all of them):
+ *   out_i = sum_j p_ij v_j,  p_i = softmax over the visible j of scale * q_i . k_j.
+ * A row that sees no key is zero; so are the rows behind cu_q[sequences]. What lies
+ * in keys or values outside a sequence is never read into its result, NaN and
+ * infinities included. Inside a sequence, V must be finite.
+ *   dim: a multiple of 8, 8 .. 128; heads / kv_heads <= 128; scale > 0.
+ *   FP16 / BF16 run on the tensor cores (probabilities rounded to the operand type
+ *   for the second product, all sums in FP32); FP32 runs on the FMA pipe.
+ *   Pointers 16-byte aligned, strides a multiple of 16 bytes
+ *   (B200_ERR_MISALIGNED_OPERAND otherwise); out is dense [tokens][heads][dim].
+ * cu_q and cu_k are device arrays of sequences + 1 offsets; they are read by the
+ * kernels only, and offsets outside the arrays do not lead to accesses outside them.
+ * `workspace` (16-byte aligned, b200_attention_prompt_workspace_bytes) holds partial
+ * results when few rows make it worth splitting the keys; it is the caller's for the
+ * duration of the call's work on `stream`, and needs no initial contents.
+ */
+typedef struct b200_attention_prompt_problem {
+  int dtype;                      /* b200_dtype of q, k, v and out */
+  int heads, kv_heads, dim;
+  int sequences;
+  int64_t q_rows, k_rows;         /* rows of the arrays */
+  b200_rows_view q, k, v;
+  void* out;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  float scale;
+  int causal;
+} b200_attention_prompt_problem;
+size_t b200_attention_prompt_workspace_bytes(const b200_attention_prompt_problem* problem);
+int b200_attention_prompt(const b200_attention_prompt_problem* problem, void* workspace, size_t workspace_bytes,
+                          b200_stream_t stream);
+
+/*
+ * One decoding step of a batch whose requests share their first `prefix` keys.
+ * Request b has one query row and sees the prefix and the first lengths[b]
+ * (clamped to 0 .. room) rows of its own part of the cache,
+ * k_cache[b * cache_batch_stride + row * row_stride + head * head_stride + d].
+ * The prefix is read once for all requests. Cache rows behind lengths[b] may hold
+ * anything. Types, limits, alignment and workspace as above; a request that sees no
+ * key gets zeros.
+ */
+typedef struct b200_attention_shared_problem {
+  int dtype;
+  int heads, kv_heads, dim;
+  int64_t batch, prefix, room;
+  b200_rows_view q, k_prefix, v_prefix, k_cache, v_cache;
+  int64_t k_batch_stride, v_batch_stride;
+  void* out;                      /* dense [batch][heads][dim] */
+  const int32_t* lengths;
+  float scale;
+} b200_attention_shared_problem;
+size_t b200_attention_shared_workspace_bytes(const b200_attention_shared_problem* problem);
+int b200_attention_shared(const b200_attention_shared_problem* problem, void* workspace, size_t workspace_bytes,
+                          b200_stream_t stream);
+
+/*
+ * y[r, n] = sum_k x[r, k] * (code[n, k] - zero[n, k / group]) * scale[n, k / group]
+ * for 1 .. 16 rows x. qweight is [n][k / 2] bytes, the even k in the low half of a
+ * byte; scales [n][k / group] of type `scale_dtype` (x's type or FP32); zeros
+ * [n][k / group] bytes (values 0 .. 15) or NULL for 8 throughout. group is a multiple
+ * of 32 that divides k. x and y are dense, of type `dtype`; x and qweight 16-byte
+ * aligned. Weights are exact in the products, sums are FP32, y is rounded once.
+ */
+typedef struct b200_matvec_w4_problem {
+  int dtype, scale_dtype;
+  int rows, n, k, group;
+  const void* x;
+  const uint8_t* qweight;
+  const void* scales;
+  const uint8_t* zeros;
+  void* y;
+} b200_matvec_w4_problem;
+int b200_matvec_w4(const b200_matvec_w4_problem* problem, b200_stream_t stream);
+
+/*
+ * Logits of a batch before the softmax. For row r and token t, in this order:
+ *   seen (in prompt or output): x = x > 0 ? x / repetition[r] : x * repetition[r]
+ *   x -= frequency[r] * (occurrences of t in output) + presence[r] * (any)
+ *   x += bias_values[r, i] for every i with bias_ids[r, i] == t
+ *   x = -infinity unless bit t % 32 of allowed[r, t / 32] is set
+ * in FP32, rounded once. Every array but `logits` and `out` may be NULL (its step is
+ * left out). Token and bias ids outside 0 .. vocab - 1 are padding. allowed_stride is
+ * 0 for one mask for all rows, else the words from one row's mask to the next's.
+ * logits and out are dense [rows][vocab], 16-byte aligned, and do not overlap.
+ */
+typedef struct b200_logits_problem {
+  int dtype;
+  int64_t rows, vocab;
+  const void* logits;
+  void* out;
+  const int32_t* prompt_tokens;   /* [rows][prompt_length] */
+  const int32_t* output_tokens;   /* [rows][output_length] */
+  int64_t prompt_length, output_length;
+  const float* repetition;        /* [rows] each */
+  const float* frequency;
+  const float* presence;
+  const int32_t* bias_ids;        /* [rows][bias_length] */
+  const float* bias_values;
+  int64_t bias_length;
+  const int32_t* allowed;
+  int64_t allowed_stride;
+} b200_logits_problem;
+int b200_process_logits(const b200_logits_problem* problem, b200_stream_t stream);
 
 /* ------------------------------------------------------ M-sharded large GEMM */
 

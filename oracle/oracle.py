@@ -95,6 +95,80 @@ def softmax_fp64(x: torch.Tensor) -> torch.Tensor:
     return torch.softmax(x.detach().cpu().double(), dim=-1).float()
 
 
+# ---------------------------------------------------------- serving operators
+# The reference has none of these; they are stated from their formulas, in FP64,
+# on whatever device the inputs are on.
+
+
+def attention_fp64(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, causal: bool):
+    """One sequence: q ``[n, heads, dim]``, k and v ``[m, kv_heads, dim]``.
+
+    Returns the output and, for error bounds, ``sum_j p_ij |v_j|`` (same shape) and
+    ``max_j scale * sum_d |q_id k_jd|`` (``[n, heads, 1]``). Query i sees the first
+    ``m - n + i + 1`` keys when causal; a row without keys is zero.
+    """
+    n, heads, _ = q.shape
+    m = k.shape[0]
+    q64 = q.double().transpose(0, 1)
+    k64, v64 = (t.double().transpose(0, 1).repeat_interleave(heads // k.shape[1], dim=0) for t in (k, v))
+    seen = torch.ones(n, m, dtype=torch.bool, device=q.device)
+    if causal:
+        seen = torch.arange(m, device=q.device)[None] <= torch.arange(n, device=q.device)[:, None] + (m - n)
+    if m == 0:
+        zero = torch.zeros(n, heads, q.shape[2], dtype=torch.float64, device=q.device)
+        return zero, zero, zero[..., :1]
+    scores = torch.where(seen, q64 @ k64.transpose(1, 2) * scale, -math.inf)
+    p = torch.where(seen.any(1)[:, None], torch.softmax(scores, dim=-1), 0.0)
+    size = torch.where(seen, q64.abs() @ k64.abs().transpose(1, 2) * scale, 0.0).amax(-1, keepdim=True)
+    return (p @ v64).transpose(0, 1), (p @ v64.abs()).transpose(0, 1), size.transpose(0, 1)
+
+
+def matvec_w4_fp64(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None):
+    """``x @ W.T`` and, for error bounds, ``|x| @ |W|.T``."""
+    n, groups = scales.shape
+    codes = torch.stack([qweight & 15, qweight >> 4], dim=-1).view(n, groups, -1).double()
+    weight = (codes - (8.0 if zeros is None else zeros.double()[..., None])) * scales.double()[..., None]
+    weight = weight.view(n, -1)
+    return x.double() @ weight.t(), x.double().abs() @ weight.abs().t()
+
+
+def process_logits_fp64(logits, prompt_tokens=None, output_tokens=None, repetition_penalty=None, frequency_penalty=None,
+                        presence_penalty=None, bias_ids=None, bias_values=None, allowed=None):
+    """Row by row and token by token, on the CPU; returns the result and the sum of the absolute terms."""
+    out = logits.detach().cpu().double().clone()
+    size = out.abs()
+    rows, vocab = out.shape
+    cpu = lambda t: None if t is None else t.detach().cpu()  # noqa: E731
+    prompt_tokens, output_tokens, bias_ids, bias_values, allowed = map(cpu, (prompt_tokens, output_tokens, bias_ids, bias_values, allowed))
+    for r in range(rows):
+        inside = lambda t: [] if t is None else [int(i) for i in t[r] if 0 <= int(i) < vocab]  # noqa: E731
+        given, made = inside(prompt_tokens), inside(output_tokens)
+        counts: dict = {}
+        for t in made:
+            counts[t] = counts.get(t, 0) + 1
+        if repetition_penalty is not None:
+            by = float(repetition_penalty[r])
+            for t in set(given) | set(made):
+                out[r, t] = out[r, t] / by if out[r, t] > 0 else out[r, t] * by
+                size[r, t] = out[r, t].abs()
+        for t, count in counts.items():
+            off = (0.0 if frequency_penalty is None else float(frequency_penalty[r]) * count)
+            off += 0.0 if presence_penalty is None else float(presence_penalty[r])
+            out[r, t] -= off
+            size[r, t] += abs(off)
+        if bias_ids is not None:
+            for t, value in zip(bias_ids[r].tolist(), bias_values[r].tolist()):
+                if 0 <= t < vocab:
+                    out[r, t] += value
+                    size[r, t] += abs(value)
+        if allowed is not None:
+            words = allowed[r if allowed.shape[0] == rows else 0].tolist()
+            for t in range(vocab):
+                if not words[t // 32] >> (t % 32) & 1:
+                    out[r, t] = -math.inf
+    return out, size
+
+
 # ------------------------------------------------------------------ tolerances
 
 

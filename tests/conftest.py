@@ -56,6 +56,73 @@ class KernelMeta(ctypes.Structure):
     ]
 
 
+class RowsView(ctypes.Structure):
+    """ctypes mirror of ``b200_rows_view``."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class PromptProblem(ctypes.Structure):
+    """ctypes mirror of ``b200_attention_prompt_problem``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int), ("heads", ctypes.c_int), ("kv_heads", ctypes.c_int), ("dim", ctypes.c_int),
+        ("sequences", ctypes.c_int), ("q_rows", ctypes.c_int64), ("k_rows", ctypes.c_int64),
+        ("q", RowsView), ("k", RowsView), ("v", RowsView), ("out", ctypes.c_void_p),
+        ("cu_q", ctypes.c_void_p), ("cu_k", ctypes.c_void_p), ("scale", ctypes.c_float), ("causal", ctypes.c_int),
+    ]
+
+
+class SharedProblem(ctypes.Structure):
+    """ctypes mirror of ``b200_attention_shared_problem``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int), ("heads", ctypes.c_int), ("kv_heads", ctypes.c_int), ("dim", ctypes.c_int),
+        ("batch", ctypes.c_int64), ("prefix", ctypes.c_int64), ("room", ctypes.c_int64),
+        ("q", RowsView), ("k_prefix", RowsView), ("v_prefix", RowsView), ("k_cache", RowsView), ("v_cache", RowsView),
+        ("k_batch_stride", ctypes.c_int64), ("v_batch_stride", ctypes.c_int64), ("out", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p), ("scale", ctypes.c_float),
+    ]
+
+
+class MatvecProblem(ctypes.Structure):
+    """ctypes mirror of ``b200_matvec_w4_problem``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int), ("scale_dtype", ctypes.c_int), ("rows", ctypes.c_int), ("n", ctypes.c_int), ("k", ctypes.c_int),
+        ("group", ctypes.c_int), ("x", ctypes.c_void_p), ("qweight", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+        ("zeros", ctypes.c_void_p), ("y", ctypes.c_void_p),
+    ]
+
+
+class LogitsProblem(ctypes.Structure):
+    """ctypes mirror of ``b200_logits_problem``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int), ("rows", ctypes.c_int64), ("vocab", ctypes.c_int64), ("logits", ctypes.c_void_p),
+        ("out", ctypes.c_void_p), ("prompt_tokens", ctypes.c_void_p), ("output_tokens", ctypes.c_void_p),
+        ("prompt_length", ctypes.c_int64), ("output_length", ctypes.c_int64), ("repetition", ctypes.c_void_p),
+        ("frequency", ctypes.c_void_p), ("presence", ctypes.c_void_p), ("bias_ids", ctypes.c_void_p),
+        ("bias_values", ctypes.c_void_p), ("bias_length", ctypes.c_int64), ("allowed", ctypes.c_void_p),
+        ("allowed_stride", ctypes.c_int64),
+    ]
+
+
+def load_serving_abi() -> ctypes.CDLL:
+    """The same library with the signatures of the serving operators declared too."""
+    lib = load_abi()
+    c_size_t, c_void_p, pointer = ctypes.c_size_t, ctypes.c_void_p, ctypes.POINTER
+    lib.b200_attention_prompt_workspace_bytes.restype = c_size_t
+    lib.b200_attention_prompt_workspace_bytes.argtypes = [pointer(PromptProblem)]
+    lib.b200_attention_prompt.argtypes = [pointer(PromptProblem), c_void_p, c_size_t, c_void_p]
+    lib.b200_attention_shared_workspace_bytes.restype = c_size_t
+    lib.b200_attention_shared_workspace_bytes.argtypes = [pointer(SharedProblem)]
+    lib.b200_attention_shared.argtypes = [pointer(SharedProblem), c_void_p, c_size_t, c_void_p]
+    lib.b200_matvec_w4.argtypes = [pointer(MatvecProblem), c_void_p]
+    lib.b200_process_logits.argtypes = [pointer(LogitsProblem), c_void_p]
+    return lib
+
+
 def load_abi() -> ctypes.CDLL:
     """Loads libb200_kernels.so and declares the signatures of its entry points."""
     if not KERNEL_LIB.exists():
