@@ -76,6 +76,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const A
   if (lane * 4 < a.dim) store_row4(a.out, a.dtype, row * a.dim + lane * 4, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
 }
 
+// FP32 operands would lose half their bits on the tensor cores; 16-bit ones lose nothing.
+bool on_tensor_cores(const AttentionArgs& a) { return a.dtype != B200_FP32; }
+
 int launch_join(const AttentionArgs& a, cudaStream_t s) {
   const int64_t blocks = (static_cast<int64_t>(a.q_rows) * a.heads + kJoinWarps - 1) / kJoinWarps;
   if (blocks > 0x7fffffffLL) return B200_ERR_INVALID_PROBLEM;
@@ -86,7 +89,9 @@ int launch_join(const AttentionArgs& a, cudaStream_t s) {
   const GemmLaunchAttributes attrs = gemm_launch_attributes(1);
   cfg.attrs = const_cast<cudaLaunchAttribute*>(attrs.list);
   cfg.numAttrs = attrs.count;
-  if (cudaLaunchKernelEx(&cfg, attention_join_kernel<kSimtKeyBlock>, a) != cudaSuccess) return launch_failed();
+  const cudaError_t rc = on_tensor_cores(a) ? cudaLaunchKernelEx(&cfg, attention_join_kernel<kUmmaKeyBlock>, a)
+                                            : cudaLaunchKernelEx(&cfg, attention_join_kernel<kSimtKeyBlock>, a);
+  if (rc != cudaSuccess) return launch_failed();
   return launch_status();
 }
 
@@ -160,7 +165,7 @@ int64_t unit_bound(const AttentionArgs& a) {
 
 void choose_form(AttentionArgs* a) {
   const int sms = sm_count() > 0 ? sm_count() : 1;
-  plan_attention_simt(a, sms);
+  on_tensor_cores(*a) ? plan_attention_umma(a, sms) : plan_attention_simt(a, sms);
   // A prompt is split when its rows alone would leave SMs without work; a decoding step always.
   const int64_t busy = (static_cast<int64_t>(a->q_rows) * a->group + a->unit_rows - 1) / a->unit_rows * a->kv_heads;
   a->split = a->kind == kShared || (busy < sms && a->k_rows > 4 * kSimtKeyBlock);
@@ -191,7 +196,9 @@ int run(AttentionArgs& a, void* workspace, size_t bytes, cudaStream_t s) {
     a.partial_ml = reinterpret_cast<float2*>(base + w.ml);
     a.partial_o = reinterpret_cast<float*>(base + w.o);
   }
-  if (const int rc = launch_attention_simt(a, s, a.kind == kPrompt ? unit_bound(a) : 0); rc != B200_OK) return rc;
+  const int64_t units = a.kind == kPrompt ? unit_bound(a) : 0;
+  const int rc = on_tensor_cores(a) ? launch_attention_umma(a, s, units) : launch_attention_simt(a, s, units);
+  if (rc != B200_OK) return rc;
   return a.split != 0 ? launch_join(a, s) : B200_OK;
 }
 

@@ -254,6 +254,9 @@ __device__ __forceinline__ int64_t partial_row(const AttentionArgs& a, const Seg
 
 // Launchers of the kernels; the key block of each is needed by the join.
 constexpr int kSimtKeyBlock = 64;
+constexpr int kUmmaKeyBlock = 128;
+int launch_attention_umma(const AttentionArgs& a, cudaStream_t s, int64_t units);
+void plan_attention_umma(AttentionArgs* a, int sms);
 int launch_attention_simt(const AttentionArgs& a, cudaStream_t s, int64_t units);
 void plan_attention_simt(AttentionArgs* a, int sms);
 

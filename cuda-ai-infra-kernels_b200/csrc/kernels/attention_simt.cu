@@ -1,4 +1,4 @@
-// Attention on the FMA pipe: any of the three types, FP32 arithmetic throughout.
+// Attention for FP32 operands, on the FMA pipe.
 //
 // One pass over the keys with a running maximum and sum: for a tile of rows (i, g) and a block of 64
 // keys, S = Q K^T, m' = max(m, rowmax S), P = 2^(S - m'), l = l 2^(m - m') + rowsum P,
@@ -13,26 +13,8 @@ namespace {
 constexpr int kKeys = kSimtKeyBlock;
 constexpr float kMinusInf = -__builtin_huge_valf();
 
-template <typename T> __device__ __forceinline__ float4 load4(const T* p);
-template <> __device__ __forceinline__ float4 load4<float>(const float* p) { return *reinterpret_cast<const float4*>(p); }
-template <> __device__ __forceinline__ float4 load4<__half>(const __half* p) {
-  const uint2 w = *reinterpret_cast<const uint2*>(p);
-  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-  return make_float4(a.x, a.y, b.x, b.y);
-}
-template <> __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p) {
-  const uint2 w = *reinterpret_cast<const uint2*>(p);
-  return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
-                     __uint_as_float(w.y & 0xffff0000u));
-}
+__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 __device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
-__device__ __forceinline__ void store4(__half* p, float4 v) {
-  reinterpret_cast<__half2*>(p)[0] = __floats2half2_rn(v.x, v.y), reinterpret_cast<__half2*>(p)[1] = __floats2half2_rn(v.z, v.w);
-}
-__device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v) {
-  reinterpret_cast<__nv_bfloat162*>(p)[0] = __floats2bfloat162_rn(v.x, v.y);
-  reinterpret_cast<__nv_bfloat162*>(p)[1] = __floats2bfloat162_rn(v.z, v.w);
-}
 
 __device__ __forceinline__ float half_warp_max(float v) {
 #pragma unroll
@@ -47,16 +29,16 @@ __device__ __forceinline__ float half_warp_sum(float v) {
 
 // Rows of `count` floats [rows][dim] -> shared [rows][pitch]; rows from `live` on become zeros, so that
 // nothing outside the sequence enters a product.
-template <typename T, int kThreads>
-__device__ __forceinline__ void stage_rows(float* dst, const T* src, int64_t stride, int rows, int live, int dim, int pitch) {
+template <int kThreads>
+__device__ __forceinline__ void stage_rows(float* dst, const float* src, int64_t stride, int rows, int live, int dim, int pitch) {
   const int quads = dim / 4;
   for (int i = threadIdx.x; i < rows * quads; i += kThreads) {
     const int r = i / quads, c = (i - r * quads) * 4;
-    store4(dst + r * pitch + c, r < live ? load4<T>(src + r * stride + c) : make_float4(0.f, 0.f, 0.f, 0.f));
+    store4(dst + r * pitch + c, r < live ? load4(src + r * stride + c) : make_float4(0.f, 0.f, 0.f, 0.f));
   }
 }
 
-template <typename T, int kRows>
+template <int kRows>
 __global__ void __launch_bounds__(kRows * 4) attention_simt_kernel(const AttentionArgs a) {
   constexpr int kThreads = kRows * 4;
   extern __shared__ __align__(16) float smem[];
@@ -81,7 +63,7 @@ __global__ void __launch_bounds__(kRows * 4) attention_simt_kernel(const Attenti
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < rows) {
         const int64_t flat = row0 + r;
-        v = load4<T>(static_cast<const T*>(a.q) + (g.seq.q_row + flat / a.group) * a.q_row + (g.head * a.group + flat % a.group) * a.q_head + c);
+        v = load4(static_cast<const float*>(a.q) + (g.seq.q_row + flat / a.group) * a.q_row + (g.head * a.group + flat % a.group) * a.q_head + c);
       }
       store4(qs + r * pitch + c, make_float4(v.x * a.scale_log2, v.y * a.scale_log2, v.z * a.scale_log2, v.w * a.scale_log2));
     }
@@ -93,14 +75,14 @@ __global__ void __launch_bounds__(kRows * 4) attention_simt_kernel(const Attenti
 #pragma unroll
     for (int i = 0; i < 4; ++i) m[i] = kMinusInf, l[i] = 0.f, o[i][0] = o[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
     const int s = g.seq.source;
-    const T* k = static_cast<const T*>(a.k[s]) + (s == 1 ? g.seq.batch * a.k_batch : 0) + g.seq.k_row * a.k_row[s] + g.head * a.k_head[s];
-    const T* v = static_cast<const T*>(a.v[s]) + (s == 1 ? g.seq.batch * a.v_batch : 0) + g.seq.k_row * a.v_row[s] + g.head * a.v_head[s];
+    const float* k = static_cast<const float*>(a.k[s]) + (s == 1 ? g.seq.batch * a.k_batch : 0) + g.seq.k_row * a.k_row[s] + g.head * a.k_head[s];
+    const float* v = static_cast<const float*>(a.v[s]) + (s == 1 ? g.seq.batch * a.v_batch : 0) + g.seq.k_row * a.v_row[s] + g.head * a.v_head[s];
     for (int b = g.block_begin; b < g.block_end; ++b) {
       const int64_t key0 = static_cast<int64_t>(b) * kKeys;
       const int live = min(kKeys, static_cast<int>(g.seq.m - key0));
       __syncthreads();
-      stage_rows<T, kThreads>(ks, k + key0 * a.k_row[s], a.k_row[s], kKeys, live, a.dim, pitch);
-      stage_rows<T, kThreads>(vs, v + key0 * a.v_row[s], a.v_row[s], kKeys, live, a.dim, pitch);
+      stage_rows<kThreads>(ks, k + key0 * a.k_row[s], a.k_row[s], kKeys, live, a.dim, pitch);
+      stage_rows<kThreads>(vs, v + key0 * a.v_row[s], a.v_row[s], kKeys, live, a.dim, pitch);
       __syncthreads();
       float x[4][4] = {};
       for (int d = 0; d < a.dim; d += 4) {
@@ -173,7 +155,7 @@ __global__ void __launch_bounds__(kRows * 4) attention_simt_kernel(const Attenti
           if (tx * 4 + 64 * c < a.dim) store4(a.partial_o + row * a.dim + tx * 4 + 64 * c, o[i][c]);
       } else {
         const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
-        T* y = static_cast<T*>(a.out) + output_row(a, g, flat) * a.dim;
+        float* y = static_cast<float*>(a.out) + output_row(a, g, flat) * a.dim;
 #pragma unroll
         for (int c = 0; c < 2; ++c)
           if (tx * 4 + 64 * c < a.dim)
@@ -187,9 +169,9 @@ constexpr size_t simt_smem_bytes(int rows, int dim) {
   return sizeof(float) * ((rows + 2 * static_cast<size_t>(kKeys)) * (dim + 4) + static_cast<size_t>(rows) * (kKeys + 4));
 }
 
-template <typename T, int kRows>
+template <int kRows>
 int launch(const AttentionArgs& a, int64_t blocks, cudaStream_t s) {
-  if (!ensure_dynamic_smem<attention_simt_kernel<T, kRows>, simt_smem_bytes(kRows, 128)>()) return B200_ERR_LAUNCH_FAILED;
+  if (!ensure_dynamic_smem<attention_simt_kernel<kRows>, simt_smem_bytes(kRows, 128)>()) return B200_ERR_LAUNCH_FAILED;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(kRows * 4);
@@ -198,13 +180,8 @@ int launch(const AttentionArgs& a, int64_t blocks, cudaStream_t s) {
   const GemmLaunchAttributes attrs = gemm_launch_attributes(1);
   cfg.attrs = const_cast<cudaLaunchAttribute*>(attrs.list);
   cfg.numAttrs = attrs.count;
-  if (cudaLaunchKernelEx(&cfg, attention_simt_kernel<T, kRows>, a) != cudaSuccess) return launch_failed();
+  if (cudaLaunchKernelEx(&cfg, attention_simt_kernel<kRows>, a) != cudaSuccess) return launch_failed();
   return launch_status();
-}
-
-template <typename T>
-int launch_rows(const AttentionArgs& a, int64_t blocks, cudaStream_t s) {
-  return a.unit_rows == 64 ? launch<T, 64>(a, blocks, s) : launch<T, 16>(a, blocks, s);
 }
 
 }  // namespace
@@ -220,11 +197,7 @@ void plan_attention_simt(AttentionArgs* a, int sms) {
 int launch_attention_simt(const AttentionArgs& a, cudaStream_t s, int64_t units) {
   const int64_t blocks = a.split != 0 ? a.ctas : units * a.kv_heads;
   if (blocks > 0x7fffffffLL) return B200_ERR_INVALID_PROBLEM;
-  switch (a.dtype) {
-    case B200_FP32: return launch_rows<float>(a, blocks, s);
-    case B200_FP16: return launch_rows<__half>(a, blocks, s);
-    default: return launch_rows<__nv_bfloat16>(a, blocks, s);
-  }
+  return a.unit_rows == 64 ? launch<64>(a, blocks, s) : launch<16>(a, blocks, s);
 }
 
 }  // namespace b200

@@ -134,6 +134,27 @@ bool make_tensor_map_strips(CUtensorMap* out, const float* base, uint64_t rows, 
   return true;
 }
 
+bool make_tensor_map_16bit(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                           const uint32_t* box, bool bf16) {
+  EncodeTiledFn encode = encode_tiled_fn();
+  if (encode == nullptr || rank < 3 || rank > 4 || reinterpret_cast<uintptr_t>(base) % 16 != 0) return false;
+  cuuint64_t d[4], st[3];
+  cuuint32_t b[4];
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    if (dims[i] == 0 || box[i] == 0 || box[i] > 256) return false;
+    d[i] = dims[i], b[i] = box[i];
+    if (i + 1 < rank) {
+      if (strides[i] % 16 != 0) return false;
+      st[i] = strides[i];
+    }
+  }
+  if (box[0] > 64) return false;   // 128 bytes: the span of the swizzle
+  return encode(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(base), d, st, b,
+                ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace b200
 
 extern "C" {
@@ -153,7 +174,7 @@ const char* b200_status_string(int status) {
 }
 
 const char* b200_build_info(void) {
-  return "b200_kernels 0.1 (sm_100a; FP32 SIMT ladder, TF32 tcgen05 GEMM, RMSNorm, softmax)";
+  return "b200_kernels 0.1 (sm_100a; FP32 SIMT ladder, TF32 tcgen05 GEMM, RMSNorm, softmax, serving operators)";
 }
 
 int b200_device_status_read(uint32_t* host_word, b200_stream_t stream) {
@@ -168,7 +189,9 @@ int b200_device_status_read(uint32_t* host_word, b200_stream_t stream) {
   if (b200::peer_sync_status_read_clear(&peer_word) != cudaSuccess) return B200_ERR_LAUNCH_FAILED;
   uint32_t row_word = 0;
   if (b200::rowops_status_read_clear(&row_word) != cudaSuccess) return B200_ERR_LAUNCH_FAILED;
-  *host_word = sgemm_word | umma_word | selftest_word | peer_word | row_word;
+  uint32_t attention_word = 0;
+  if (b200::attention_status_read_clear(&attention_word) != cudaSuccess) return B200_ERR_LAUNCH_FAILED;
+  *host_word = sgemm_word | umma_word | selftest_word | peer_word | row_word | attention_word;
   return *host_word == 0 ? B200_OK : B200_ERR_DEVICE_TIMEOUT;
 }
 

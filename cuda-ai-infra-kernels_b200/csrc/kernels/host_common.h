@@ -100,6 +100,7 @@ cudaError_t umma_status_read_clear(uint32_t* word);
 cudaError_t selftest_status_read_clear(uint32_t* word);
 cudaError_t peer_sync_status_read_clear(uint32_t* word);
 cudaError_t rowops_status_read_clear(uint32_t* word);
+cudaError_t attention_status_read_clear(uint32_t* word);
 
 // k128BAtom32B: 128-byte span swizzled in 32-byte granules (what an MN-major
 // 32-bit tcgen05 operand needs); k128B: the usual 16-byte granules.
@@ -112,6 +113,12 @@ enum class Swizzle { kNone, k128B, k128BAtom32B };
 // multiple of 16 (and <= 128 bytes with either 128-byte swizzle), boxes <= 256.
 bool make_tensor_map_2d(CUtensorMap* out, const float* base, uint64_t rows, uint64_t cols,
                         uint64_t ld, uint32_t box_rows, uint32_t box_cols, Swizzle swizzle);
+
+// 16-bit array of rank 3 or 4, innermost dimension first; strides (bytes, multiples of 16) of the
+// outer dimensions, a box of at most 64 x 256 x ... elements in the 128-byte swizzle. Parts of a box
+// outside the array read as zero. Encoded on every call.
+bool make_tensor_map_16bit(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                           const uint32_t* box, bool bf16);
 
 // Row-major FP32 matrix [rows][cols] (cols a multiple of 32) viewed as
 // [cols / 32][rows][32]: a box of `box_groups` x `box_rows` x 32 gathers
