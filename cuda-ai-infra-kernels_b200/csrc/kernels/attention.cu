@@ -1,5 +1,5 @@
-// Entry points of the attention operators: checks, choice of the form (direct or split), workspace
-// layout, and the pass that joins the partial results of the split form.
+// Entry points of the attention operators: checks, workspace layout, and the passes that join partial
+// results.
 #include "attention.cuh"
 
 namespace b200 {
@@ -20,79 +20,120 @@ __device__ __forceinline__ void store_row4(void* out, int dtype, int64_t at, flo
   }
 }
 
-// One warp per output row: O = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over the partial results
-// c of the row, in a fixed order. A partial result with l = 0 saw no key; its O is not read.
-template <int kKeyBlock>
-__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const AttentionArgs a) {
-  grid_launch_dependents();
-  grid_dependency_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kJoinWarps + (threadIdx.x >> 5);
-  if (row >= static_cast<int64_t>(a.q_rows) * a.heads) return;
-  const int q_row = static_cast<int>(row / a.heads), head = static_cast<int>(row % a.heads) / a.group;
-  const int g = static_cast<int>(row % a.heads) - head * a.group;
-
+// Joins the partial results c of one row, a warp per row, in CTA order:
+// O = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c. One with l = 0 saw no key; its O is not read.
+struct RowJoin {
   float top = kMinusInf, total = 0.f;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int64_t per = a.plan[0];
-  const auto join = [&](int s) {
-    const Sequence seq = sequence_of(a, s);
-    const int64_t flat = static_cast<int64_t>(q_row - seq.q_row) * a.group + g;
-    const int unit = static_cast<int>(flat / a.unit_rows);
-    if (q_row < seq.q_row || q_row - seq.q_row >= seq.n || seq.m == 0) return;
-    const int blocks = unit_blocks<kKeyBlock>(a, seq, unit);
-    if (blocks == 0) return;
-    int64_t first = a.plan[1 + s] + head * head_blocks<kKeyBlock>(a, seq);
-    for (int t = 0; t < unit; ++t) first += unit_blocks<kKeyBlock>(a, seq, t);
-    const int c0 = static_cast<int>(first / per), c1 = static_cast<int>((first + blocks - 1) / per);
-    for (int c = c0; c <= c1; ++c) {
-      const int64_t at = c == c0 ? row + (seq.source == 1 ? static_cast<int64_t>(a.q_rows) * a.heads : 0)
-                                 : a.natural_rows + static_cast<int64_t>(c) * a.unit_rows + (flat - static_cast<int64_t>(unit) * a.unit_rows);
-      const float2 ml = a.partial_ml[at];
-      if (ml.y == 0.f) continue;
-      const float next = fmaxf(top, ml.x);
-      const float base = next == kMinusInf ? 0.f : next;   // maxima of -infinity with l != 0: NaN rows
-      const float keep = exp2f(top - base), add = exp2f(ml.x - base);
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (lane * 4 < a.dim) v = *reinterpret_cast<const float4*>(a.partial_o + at * a.dim + lane * 4);
-      sum = make_float4(sum.x * keep + v.x * add, sum.y * keep + v.y * add, sum.z * keep + v.z * add, sum.w * keep + v.w * add);
-      total = total * keep + ml.y * add;
-      top = next;
-    }
-  };
-  if (a.kind == kShared) {
-    join(0);
-    join(1 + q_row);
-  } else {
-    int lo = 0, hi = a.sequences + 1;   // the last offset that is not behind the row
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (__ldg(a.cu_q + mid) <= q_row) lo = mid;
-      else hi = mid;
-    }
-    if (lo < a.sequences) join(lo);
+
+  __device__ __forceinline__ void add(const AttentionArgs& a, int64_t at, int lane) {
+    const float2 ml = a.partial_ml[at];
+    if (ml.y == 0.f) return;
+    const float next = fmaxf(top, ml.x);
+    const float base = next == kMinusInf ? 0.f : next;   // maxima of -infinity with l != 0: NaN rows
+    const float keep = exp2f(top - base), more = exp2f(ml.x - base);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (lane * 4 < a.dim) v = *reinterpret_cast<const float4*>(a.partial_o + at * a.dim + lane * 4);
+    sum = make_float4(sum.x * keep + v.x * more, sum.y * keep + v.y * more, sum.z * keep + v.z * more, sum.w * keep + v.w * more);
+    total = total * keep + ml.y * more;
+    top = next;
   }
-  const float inv = total == 0.f ? 0.f : 1.f / total;
-  if (lane * 4 < a.dim) store_row4(a.out, a.dtype, row * a.dim + lane * 4, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+  __device__ __forceinline__ void store(const AttentionArgs& a, int64_t row, int lane) const {
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    if (lane * 4 < a.dim) store_row4(a.out, a.dtype, row * a.dim + lane * 4, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+  }
+};
+
+// Prompt calls: block (c, y) handles rows y, y + gridDim.y, ... (in groups of a warp each) of the unit
+// that boundary c cuts, if c is the first that does.
+template <int kKeys>
+__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_cuts_kernel(const AttentionArgs a) {
+  __shared__ WorkScratch scratch;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int cta = blockIdx.x + 1;
+  const WorkStart start = find_range<kKeys, kJoinWarps * 32>(a, &scratch, cta);
+  if (start.sequence < 0 || start.block == 0 || start.before / start.per != cta - 1) return;
+  const Sequence seq = sequence_of(a, start.sequence);
+  const int last = static_cast<int>((start.before + unit_weight<kKeys>(a, seq, start.unit) - 1) / start.per);
+  const int row0 = start.unit * a.unit_rows;
+  const int rows = min(a.unit_rows, seq.n * a.group - row0);
+  const int lane = threadIdx.x & 31;
+  for (int r = blockIdx.y * kJoinWarps + (threadIdx.x >> 5); r < rows; r += gridDim.y * kJoinWarps) {
+    RowJoin join;
+    const int64_t out = output_row(a, seq, start.head, row0 + r);
+    join.add(a, opened_row(a, seq, out, cta - 1, r), lane);
+    for (int c = cta; c <= last; ++c) join.add(a, continued_row(a, c, r), lane);
+    join.store(a, out, lane);
+  }
+}
+
+// Shared-prefix calls: a warp per row, which has a part over the prefix and one over its own keys. All
+// rows of a block belong to one request (blockIdx.x); the block finds the requests' first blocks by
+// itself.
+template <int kKeys>
+__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_rows_kernel(const AttentionArgs a) {
+  __shared__ int64_t sums[2][kJoinWarps];
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, request = blockIdx.x;
+  const auto head_size = [&](int s) { return head_weight<kKeys>(a, sequence_of(a, s)); };
+  int64_t all = 0, before = 0;   // blocks of a key head: of all sequences, and of those ahead of this request
+  for (int s = threadIdx.x; s < a.sequences; s += kJoinWarps * 32) {
+    const int64_t size = head_size(s);
+    all += size;
+    if (s < request + 1) before += size;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o), before += __shfl_xor_sync(0xffffffffu, before, o);
+  if (lane == 0) sums[0][threadIdx.x >> 5] = all, sums[1][threadIdx.x >> 5] = before;
+  __syncthreads();
+  all = before = 0;
+  for (int w = 0; w < kJoinWarps; ++w) all += sums[0][w], before += sums[1][w];
+  const int64_t per = quotient(a.kv_heads * all + a.ctas - 1, a.ctas);
+  const Sequence prefix = sequence_of(a, 0), own = sequence_of(a, 1 + request);
+  for (int h = blockIdx.y * kJoinWarps + (threadIdx.x >> 5); h < a.heads; h += gridDim.y * kJoinWarps) {
+    const int head = h / a.group, g = h - head * a.group;
+    RowJoin join;
+    const int64_t out = static_cast<int64_t>(request) * a.heads + h;
+    const auto part = [&](const Sequence& seq, int64_t first_of_sequence, int flat) {
+      const int unit = flat / a.unit_rows, row = flat - unit * a.unit_rows;
+      const int blocks = unit_blocks<kKeys>(a, seq, unit);
+      if (blocks == 0) return;
+      const int64_t first = first_of_sequence + head * head_weight<kKeys>(a, seq) + weight_before<kKeys>(a, seq, unit);
+      const int c0 = static_cast<int>(quotient(first, per)), c1 = static_cast<int>(quotient(first + blocks - 1, per));
+      join.add(a, opened_row(a, seq, out, c0, row), lane);
+      for (int c = c0 + 1; c <= c1; ++c) join.add(a, continued_row(a, c, row), lane);
+    };
+    part(prefix, 0, request * a.group + g);
+    part(own, a.kv_heads * before, g);
+    join.store(a, out, lane);
+  }
 }
 
 // FP32 operands would lose half their bits on the tensor cores; 16-bit ones lose nothing.
 bool on_tensor_cores(const AttentionArgs& a) { return a.dtype != B200_FP32; }
 
-int launch_join(const AttentionArgs& a, cudaStream_t s) {
-  const int64_t blocks = (static_cast<int64_t>(a.q_rows) * a.heads + kJoinWarps - 1) / kJoinWarps;
-  if (blocks > 0x7fffffffLL) return B200_ERR_INVALID_PROBLEM;
+template <typename Kernel>
+int launch_join(Kernel kernel, dim3 grid, const AttentionArgs& a, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = s;
   const GemmLaunchAttributes attrs = gemm_launch_attributes(1);
   cfg.attrs = const_cast<cudaLaunchAttribute*>(attrs.list);
   cfg.numAttrs = attrs.count;
-  const cudaError_t rc = on_tensor_cores(a) ? cudaLaunchKernelEx(&cfg, attention_join_kernel<kUmmaKeyBlock>, a)
-                                            : cudaLaunchKernelEx(&cfg, attention_join_kernel<kSimtKeyBlock>, a);
-  if (rc != cudaSuccess) return launch_failed();
+  if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) return launch_failed();
   return launch_status();
+}
+
+template <int kKeys>
+int join(const AttentionArgs& a, cudaStream_t s) {
+  if (a.kind == kShared) {
+    const unsigned share = static_cast<unsigned>((a.heads + kJoinWarps - 1) / kJoinWarps);
+    return launch_join(attention_join_rows_kernel<kKeys>, dim3(static_cast<unsigned>(a.q_rows), share < 32 ? share : 32), a, s);
+  }
+  return a.ctas < 2 ? B200_OK : launch_join(attention_join_cuts_kernel<kKeys>, dim3(static_cast<unsigned>(a.ctas) - 1, 8), a, s);
 }
 
 // ------------------------------------------------------------------- arguments
@@ -118,13 +159,16 @@ int check_view(const b200_rows_view& v, int64_t rows, size_t element) {
   return B200_OK;
 }
 
-constexpr int64_t kMostRows = int64_t{1} << 30;   // rows are counted in 32 bits on the device
+// Rows of an array, and rows of a key head (tokens times group), are counted in 32 bits on the device.
+constexpr int64_t kMostRows = int64_t{1} << 30;
 
 // What launches and workspace sizes follow from; host only.
 int make_args(const b200_attention_prompt_problem& q, AttentionArgs* a) {
   if (const int rc = check_common(q.dtype, q.heads, q.kv_heads, q.dim, q.scale); rc != B200_OK) return rc;
   if (q.sequences < 0 || q.q_rows < 0 || q.k_rows < 0) return B200_ERR_INVALID_ARGUMENT;
-  if (q.q_rows > kMostRows || q.k_rows > kMostRows || q.sequences > kMostRows) return B200_ERR_INVALID_PROBLEM;
+  if (q.q_rows > kMostRows || q.k_rows > kMostRows || q.sequences > kMostRows ||
+      q.q_rows * (q.heads / q.kv_heads) > kMostRows)
+    return B200_ERR_INVALID_PROBLEM;
   *a = AttentionArgs{};
   a->kind = kPrompt, a->dtype = q.dtype, a->sequences = q.sequences;
   a->q_rows = static_cast<int>(q.q_rows), a->k_rows = static_cast<int>(q.k_rows);
@@ -134,14 +178,14 @@ int make_args(const b200_attention_prompt_problem& q, AttentionArgs* a) {
   a->k[0] = q.k.data, a->k_row[0] = q.k.row_stride, a->k_head[0] = q.k.head_stride;
   a->v[0] = q.v.data, a->v_row[0] = q.v.row_stride, a->v_head[0] = q.v.head_stride;
   a->out = q.out, a->cu_q = q.cu_q, a->cu_k = q.cu_k;
-  a->natural_rows = static_cast<int64_t>(a->q_rows) * a->heads;
   return B200_OK;
 }
 
 int make_args(const b200_attention_shared_problem& q, AttentionArgs* a) {
   if (const int rc = check_common(q.dtype, q.heads, q.kv_heads, q.dim, q.scale); rc != B200_OK) return rc;
   if (q.batch < 0 || q.prefix < 0 || q.room < 0 || q.k_batch_stride < 0 || q.v_batch_stride < 0) return B200_ERR_INVALID_ARGUMENT;
-  if (q.batch > kMostRows || q.prefix > kMostRows || q.room > kMostRows) return B200_ERR_INVALID_PROBLEM;
+  if (q.batch > kMostRows || q.prefix > kMostRows || q.room > kMostRows || q.batch * (q.heads / q.kv_heads) > kMostRows)
+    return B200_ERR_INVALID_PROBLEM;
   *a = AttentionArgs{};
   a->kind = kShared, a->dtype = q.dtype, a->sequences = static_cast<int>(q.batch) + 1;
   a->q_rows = static_cast<int>(q.batch), a->k_rows = static_cast<int>(q.prefix), a->room = static_cast<int>(q.room);
@@ -153,61 +197,63 @@ int make_args(const b200_attention_shared_problem& q, AttentionArgs* a) {
   a->k[1] = q.k_cache.data, a->k_row[1] = q.k_cache.row_stride, a->k_head[1] = q.k_cache.head_stride, a->k_batch = q.k_batch_stride;
   a->v[1] = q.v_cache.data, a->v_row[1] = q.v_cache.row_stride, a->v_head[1] = q.v_cache.head_stride, a->v_batch = q.v_batch_stride;
   a->out = q.out, a->lengths = q.lengths;
-  a->natural_rows = 2 * static_cast<int64_t>(a->q_rows) * a->heads;   // prefix parts, own parts
   return B200_OK;
 }
 
-// Upper bound of the units of one key head of a prompt call: each sequence, and the rows behind
-// them, rounds up once.
-int64_t unit_bound(const AttentionArgs& a) {
-  return static_cast<int64_t>(a.q_rows) * a.group / a.unit_rows + a.sequences + 1;
-}
-
-void choose_form(AttentionArgs* a) {
+// Decomposition, without the lengths: returns whether there may be partial results.
+bool plan(AttentionArgs* a) {
   const int sms = sm_count() > 0 ? sm_count() : 1;
   on_tensor_cores(*a) ? plan_attention_umma(a, sms) : plan_attention_simt(a, sms);
-  // A prompt is split when its rows alone would leave SMs without work; a decoding step always.
-  const int64_t busy = (static_cast<int64_t>(a->q_rows) * a->group + a->unit_rows - 1) / a->unit_rows * a->kv_heads;
-  a->split = a->kind == kShared || (busy < sms && a->k_rows > 4 * kSimtKeyBlock);
+  a->token_shift = log2_or_minus_one(a->tokens);
+  const int64_t keys = on_tensor_cores(*a) ? kUmmaKeyBlock : kSimtKeyBlock;
+  const auto blocks = [&](int64_t rows) { return (rows + keys - 1) / keys; };
+  if (a->kind == kShared) {
+    // Never more ranges than blocks.
+    const int64_t own = (a->group + a->unit_rows - 1) / a->unit_rows * static_cast<int64_t>(a->q_rows) * blocks(a->room);
+    const int64_t prefix = (static_cast<int64_t>(a->q_rows) * a->group + a->unit_rows - 1) / a->unit_rows * blocks(a->k_rows);
+    const int64_t most = (own + prefix) * a->kv_heads;
+    if (most < a->ctas) a->ctas = static_cast<int>(most > 0 ? most : 1);
+    return true;
+  }
+  // Each sequence, and the rows behind them, rounds up once.
+  const int64_t units = (static_cast<int64_t>(a->q_rows) * a->group / a->unit_rows + a->sequences + 1) * a->kv_heads;
+  const int64_t longest = blocks(a->k_rows) > 0 ? blocks(a->k_rows) : 1;
+  if (units < a->ctas && units * longest < a->ctas) a->ctas = static_cast<int>(units * longest);
+  return longest > 1;   // units of one block are never cut
 }
 
 struct Workspace {
-  size_t plan, ml, o, total;
+  size_t o, total;   // maxima and denominators first
 };
 Workspace workspace_of(const AttentionArgs& a) {
   const auto round = [](size_t v) { return (v + 255) & ~size_t{255}; };
-  if (a.split == 0) return Workspace{0, 0, 0, 0};
-  const size_t rows = static_cast<size_t>(a.natural_rows) + static_cast<size_t>(a.ctas) * a.unit_rows;
+  const size_t cuts = static_cast<size_t>(a.ctas) * a.unit_rows;
+  const size_t rows = cuts + (a.kind == kShared ? 2 * static_cast<size_t>(a.q_rows) * a.heads : cuts);
   Workspace w{};
-  w.ml = round((static_cast<size_t>(a.sequences) + 3) * sizeof(int64_t));
-  w.o = w.ml + round(rows * sizeof(float2));
+  w.o = round(rows * sizeof(float2));
   w.total = w.o + round(rows * a.dim * sizeof(float));
   return w;
 }
 
 int run(AttentionArgs& a, void* workspace, size_t bytes, cudaStream_t s) {
-  choose_form(&a);
-  const Workspace w = workspace_of(a);
-  if (w.total > 0) {
+  const bool partial = plan(&a);
+  if (partial) {
+    const Workspace w = workspace_of(a);
     if (workspace == nullptr || bytes < w.total) return B200_ERR_INVALID_ARGUMENT;
     if (!aligned16(workspace)) return B200_ERR_MISALIGNED_OPERAND;
-    uint8_t* base = static_cast<uint8_t*>(workspace);
-    a.plan = reinterpret_cast<int64_t*>(base);
-    a.partial_ml = reinterpret_cast<float2*>(base + w.ml);
-    a.partial_o = reinterpret_cast<float*>(base + w.o);
+    a.partial_ml = static_cast<float2*>(workspace);
+    a.partial_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + w.o);
   }
-  const int64_t units = a.kind == kPrompt ? unit_bound(a) : 0;
-  const int rc = on_tensor_cores(a) ? launch_attention_umma(a, s, units) : launch_attention_simt(a, s, units);
-  if (rc != B200_OK) return rc;
-  return a.split != 0 ? launch_join(a, s) : B200_OK;
+  const int rc = on_tensor_cores(a) ? launch_attention_umma(a, s) : launch_attention_simt(a, s);
+  if (rc != B200_OK || !partial) return rc;
+  return on_tensor_cores(a) ? join<kUmmaKeyBlock>(a, s) : join<kSimtKeyBlock>(a, s);
 }
 
 template <class Problem>
 size_t workspace_bytes(const Problem* problem) {
   AttentionArgs a;
   if (problem == nullptr || make_args(*problem, &a) != B200_OK) return 0;
-  choose_form(&a);
-  return workspace_of(a).total;
+  return plan(&a) ? workspace_of(a).total : 0;
 }
 
 }  // namespace

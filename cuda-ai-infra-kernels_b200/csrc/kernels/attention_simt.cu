@@ -52,24 +52,24 @@ __global__ void __launch_bounds__(kRows * 4) attention_simt_kernel(const Attenti
   grid_launch_dependents();
   grid_dependency_wait();
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  SegmentWalk<kKeys> walk(a, find_attention_work<kKeys, kThreads>(a, &scratch));
+  SegmentWalk<kKeys> walk(a, find_range<kKeys, kThreads>(a, &scratch, blockIdx.x));
   Segment g;
   while (walk.next(&g)) {
-    const int64_t row0 = static_cast<int64_t>(g.unit) * a.unit_rows;
-    const int rows = static_cast<int>(min(static_cast<int64_t>(kRows), static_cast<int64_t>(g.seq.n) * a.group - row0));
+    const int row0 = g.unit * a.unit_rows;
+    const int rows = min(a.unit_rows, g.seq.n * a.group - row0);
     __syncthreads();   // the last segment's readers are done
     for (int i = threadIdx.x; i < kRows * (a.dim / 4); i += kThreads) {
       const int r = i / (a.dim / 4), c = (i - r * (a.dim / 4)) * 4;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < rows) {
-        const int64_t flat = row0 + r;
-        v = load4(static_cast<const float*>(a.q) + (g.seq.q_row + flat / a.group) * a.q_row + (g.head * a.group + flat % a.group) * a.q_head + c);
+        const int token = (row0 + r) / a.group, head = g.head * a.group + (row0 + r - token * a.group);
+        v = load4(static_cast<const float*>(a.q) + static_cast<int64_t>(g.seq.q_row + token) * a.q_row + head * a.q_head + c);
       }
       store4(qs + r * pitch + c, make_float4(v.x * a.scale_log2, v.y * a.scale_log2, v.z * a.scale_log2, v.w * a.scale_log2));
     }
     int seen[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) seen[i] = visible_keys(a, g.seq, static_cast<int>((row0 + ty * 4 + i) / a.group));
+    for (int i = 0; i < 4; ++i) seen[i] = visible_keys(a, g.seq, (row0 + ty * 4 + i) / a.group);
     float m[4], l[4];
     float4 o[4][2];
 #pragma unroll
@@ -146,16 +146,16 @@ __global__ void __launch_bounds__(kRows * 4) attention_simt_kernel(const Attenti
     for (int i = 0; i < 4; ++i) {
       const int r = ty * 4 + i;
       if (r >= rows) continue;
-      const int64_t flat = row0 + r;
-      if (a.split != 0) {
-        const int64_t row = partial_row(a, g, flat);
+      const int64_t out = output_row(a, g.seq, g.head, row0 + r);
+      if (is_partial(a, g)) {
+        const int64_t row = partial_row(a, g, out, r);
         if (tx == 0) a.partial_ml[row] = make_float2(m[i], l[i]);
 #pragma unroll
         for (int c = 0; c < 2; ++c)
           if (tx * 4 + 64 * c < a.dim) store4(a.partial_o + row * a.dim + tx * 4 + 64 * c, o[i][c]);
       } else {
         const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
-        float* y = static_cast<float*>(a.out) + output_row(a, g, flat) * a.dim;
+        float* y = static_cast<float*>(a.out) + out * a.dim;
 #pragma unroll
         for (int c = 0; c < 2; ++c)
           if (tx * 4 + 64 * c < a.dim)
@@ -170,10 +170,10 @@ constexpr size_t simt_smem_bytes(int rows, int dim) {
 }
 
 template <int kRows>
-int launch(const AttentionArgs& a, int64_t blocks, cudaStream_t s) {
+int launch(const AttentionArgs& a, cudaStream_t s) {
   if (!ensure_dynamic_smem<attention_simt_kernel<kRows>, simt_smem_bytes(kRows, 128)>()) return B200_ERR_LAUNCH_FAILED;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.gridDim = dim3(static_cast<unsigned>(a.ctas));
   cfg.blockDim = dim3(kRows * 4);
   cfg.dynamicSmemBytes = simt_smem_bytes(kRows, a.dim);
   cfg.stream = s;
@@ -186,18 +186,18 @@ int launch(const AttentionArgs& a, int64_t blocks, cudaStream_t s) {
 
 }  // namespace
 
-// Rows of a unit and, for the split form, how many CTAs share the blocks.
 void plan_attention_simt(AttentionArgs* a, int sms) {
-  // Tiles of 16 rows where the rows of a sequence would leave most of a 64-row tile empty.
+  // Tiles of 16 rows where the rows of a sequence would leave most of a 64-row tile empty; whole tokens
+  // where the group allows it.
   const int64_t rows_per_sequence = a->kind == kShared ? a->group : static_cast<int64_t>(a->q_rows) * a->group / (a->sequences > 0 ? a->sequences : 1);
-  a->unit_rows = rows_per_sequence <= 16 ? 16 : 64;
-  a->ctas = sms * (a->unit_rows == 16 ? 3 : 2);
+  const int tile = rows_per_sequence <= 16 ? 16 : 64;
+  a->tokens = tile / a->group;
+  a->unit_rows = a->tokens > 0 ? a->tokens * a->group : tile;
+  a->ctas = sms * (tile == 16 ? 3 : 2);
 }
 
-int launch_attention_simt(const AttentionArgs& a, cudaStream_t s, int64_t units) {
-  const int64_t blocks = a.split != 0 ? a.ctas : units * a.kv_heads;
-  if (blocks > 0x7fffffffLL) return B200_ERR_INVALID_PROBLEM;
-  return a.unit_rows == 64 ? launch<64>(a, blocks, s) : launch<16>(a, blocks, s);
+int launch_attention_simt(const AttentionArgs& a, cudaStream_t s) {
+  return a.unit_rows > 16 ? launch<64>(a, s) : launch<16>(a, s);
 }
 
 }  // namespace b200

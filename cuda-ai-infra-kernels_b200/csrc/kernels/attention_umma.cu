@@ -19,8 +19,11 @@
 // P <= 256 and nothing overflows; the quotient is the same.
 //
 // Warps 0-3 and 4-7: streams 0 and 1, warp w owning TMEM lanes 32 (w mod 4) ... Warp 8: copies (TMA).
-// Warp 9: issues the MMAs, and clears the value rows behind the last key of a sequence, which hold
-// foreign data that 0 * NaN would let in.
+// Warps 9 and 10: one MMA-issuing thread per stream (a lone thread spends as long on barriers and
+// commits as the tensor pipe on its products, and held the pipe at half its rate; with two, one
+// waits while the other issues). Warp 11 walks the CTA's segments and hands them out through a small
+// ring, so that nobody else carries the walk's state or waits for its arithmetic; and it clears
+// the value rows behind the last key of a sequence, which hold foreign data that 0 * NaN would let in.
 #include "attention.cuh"
 
 namespace b200 {
@@ -29,7 +32,10 @@ cudaError_t attention_status_read_clear(uint32_t* word) { return status_word_rea
 
 namespace {
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;
+// Registers: 168 per thread at launch; a softmax thread holds a row of 128 scores and takes more.
+constexpr int kSoftmaxRegisters = 216, kOtherRegisters = 72;
+static_assert(256 * kSoftmaxRegisters + 128 * kOtherRegisters <= kThreads * 168, "registers of the CTA");
 constexpr int kTile = 128;          // rows of a tile, keys of a block
 constexpr float kMinusInf = -__builtin_huge_valf();
 constexpr float kLazy = 8.f;        // growth of a maximum, in powers of two, that forces a rescale
@@ -45,18 +51,51 @@ struct Smem {
   static constexpr int kHalves = kDim / 64;                 // 128-byte spans per row
   static constexpr int kHalfBytes = kTile * 128;
   static constexpr int kTileBytes = kHalves * kHalfBytes;   // a tile of Q, a block of K or of V
-  static constexpr int kSlots = kDim == 128 ? 5 : 10;
-  static constexpr size_t kTiles = (2 + kSlots) * static_cast<size_t>(kTileBytes);
+  static constexpr int kSlots = kDim == 128 ? 4 : 8;
+  static constexpr size_t kStaging = (2 + kSlots) * static_cast<size_t>(kTileBytes);   // 4 KiB per softmax warp
+  static constexpr size_t kTiles = kStaging + 8 * 4096;
 };
 
+// What the roles need of a segment (attention.cuh), for a unit of whole tokens.
+struct SegmentEntry {
+  int blocks;              // of keys; -1: no more segments
+  int pair;                // two row tiles over all blocks; else one tile, even and odd blocks
+  int q_row, tokens;       // the unit's first query row, and tokens from there to the sequence's end
+  int k_row, batch, source, head;   // k_row: of the first block
+  int keys, ahead;         // from the first block on: keys of the sequence; keys that token t of the unit sees
+                           // are ahead + t, cut to 0 .. keys
+  int live_keys;           // of the last block
+  int partial;
+  int64_t partial_row;     // of the unit's first row, where rows follow one another; -1: by output row
+};
+constexpr int kEntries = 4;
+
 struct Shared {   // behind the tiles
-  uint64_t full[10], empty[10];
+  uint64_t full[8], empty[8], raw[8];
+  uint64_t entry_full[kEntries], entry_empty[kEntries];
   uint64_t q_full, q_empty;
   uint64_t s_full[2], p_ready[2];
-  uint64_t o_full, o_empty;
+  uint64_t o_full[2], o_empty[2];
+  uint64_t exchanged;          // eight warps have written, then eight have read
   uint32_t tmem;
+  SegmentEntry entries[kEntries];
   float2 exchange[2][kTile];   // maximum and denominator of both streams
   WorkScratch scratch;
+};
+constexpr int kEntryReaders = 1 + 2 + 8;
+
+__device__ __forceinline__ int items_of(const SegmentEntry& e, int s) { return e.pair != 0 ? e.blocks : (e.blocks + 1 - s) / 2; }
+
+// A role's place in the ring of segments. Called by whole warps or by single threads.
+struct EntryReader {
+  Shared* b;
+  uint32_t count = 0;
+  bool ok = true;
+  __device__ __forceinline__ const SegmentEntry* wait() {
+    ok = ok && mbar_wait(&b->entry_full[count % kEntries], count / kEntries & 1, kSiteAttention);
+    return &b->entries[count % kEntries];
+  }
+  __device__ __forceinline__ void release() { mbar_arrive(&b->entry_empty[count++ % kEntries]); }
 };
 
 // After tcgen05.wait::ld: keeps uses of loaded registers behind the wait.
@@ -90,142 +129,180 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   }
 }
 
-// How the two streams share a segment.
-struct Shape {
-  int blocks;
-  bool pair;   // two row tiles over all blocks; else one tile, even and odd blocks
-  __device__ __forceinline__ int items() const { return pair ? 2 * blocks : blocks; }
-  __device__ __forceinline__ int of_stream(int s) const { return pair ? blocks : (blocks + 1 - s) / 2; }
-};
-__device__ __forceinline__ Shape shape_of(const AttentionArgs& a, const Segment& g) {
-  const int64_t rows = static_cast<int64_t>(g.seq.n) * a.group - static_cast<int64_t>(g.unit) * a.unit_rows;
-  return Shape{g.block_end - g.block_begin, rows > a.unit_rows / 2};
+// ------------------------------------------------------------------------ segments, value rows
+
+template <int kDim>
+__device__ __forceinline__ void segment_role(const UmmaAttentionArgs& p, const WorkStart& start, uint8_t* smem, Shared* b) {
+  using S = Smem<kDim>;
+  const AttentionArgs& a = p.a;
+  const int lane = threadIdx.x & 31;
+  SegmentWalk<kUmmaKeyBlock> walk(a, start);
+  Segment g;
+  bool ok = true;
+  // Blocks whose last rows have to be cleared, at most kDelay segments behind the newest: the slot of
+  // the ring and the live rows.
+  constexpr uint32_t kDelay = 2;
+  int slot_of[kDelay] = {-1, -1}, live_of[kDelay] = {0, 0};
+  uint32_t loads = 0, raw_phase = 0;
+  const auto clear = [&](int i) {
+    const int slot = slot_of[i];
+    if (slot < 0) return;
+    slot_of[i] = -1;
+    ok = __all_sync(0xffffffffu, ok && mbar_wait(&b->raw[slot], raw_phase >> slot & 1, kSiteAttention));
+    raw_phase ^= 1u << slot;
+    if (!ok) return;
+    uint8_t* v = smem + (2 + slot) * S::kTileBytes;
+    for (int j = live_of[i] * 8 + lane; j < kTile * 8; j += 32)
+#pragma unroll
+      for (int h = 0; h < S::kHalves; ++h) *reinterpret_cast<uint4*>(v + h * S::kHalfBytes + j * 16) = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&b->full[slot]);
+  };
+  for (uint32_t count = 0;; ++count) {
+    const bool more = walk.next(&g);
+    ok = __all_sync(0xffffffffu, ok && mbar_wait(&b->entry_empty[count % kEntries], (count / kEntries & 1) ^ 1, kSiteAttention));
+    SegmentEntry e{};
+    if (more) {
+      const int first = g.block_begin * kTile, token0 = g.unit * a.tokens;
+      e.blocks = g.block_end - g.block_begin;
+      e.tokens = g.seq.n - token0;
+      e.pair = e.tokens > a.tokens / 2;
+      e.q_row = g.seq.q_row + token0, e.k_row = g.seq.k_row + first;
+      e.batch = g.seq.batch, e.source = g.seq.source, e.head = g.head;
+      e.keys = g.seq.m - first;
+      e.ahead = a.kind == kShared || a.causal == 0 ? e.keys : g.seq.m - g.seq.n + token0 + 1 - first;
+      e.live_keys = min(kTile, g.seq.m - (g.block_end - 1) * kTile);
+      e.partial = is_partial(a, g);
+      e.partial_row = g.opens && a.kind == kShared ? -1 : partial_row(a, g, 0, 0);
+    } else {
+      e.blocks = -1;
+    }
+    if (lane == 0) {
+      b->entries[count % kEntries] = e;
+      mbar_arrive(&b->entry_full[count % kEntries]);
+    }
+    clear(count % kDelay);   // the segment before the last one
+    if (!more) {
+      clear((count + 1) % kDelay);
+      return;
+    }
+    if (e.blocks > 0) {
+      loads += 2 * e.blocks;
+      if (e.live_keys < kTile) slot_of[count % kDelay] = (loads - 1) % S::kSlots, live_of[count % kDelay] = e.live_keys;
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------- copies
 
 template <int kDim>
-__device__ __forceinline__ void copy_role(const UmmaAttentionArgs& p, const WorkStart& start, uint8_t* smem, Shared* b) {
+__device__ __forceinline__ void copy_role(const UmmaAttentionArgs& p, uint8_t* smem, Shared* b) {
   using S = Smem<kDim>;
   const AttentionArgs& a = p.a;
-  const int tokens = a.unit_rows / 2 / a.group;   // of a tile
-  SegmentWalk<kUmmaKeyBlock> walk(a, start);
-  Segment g;
-  bool ok = true;
+  const int tokens = a.tokens / 2;   // of a tile
+  EntryReader reader{b};
   uint32_t load = 0, segment = 0;
-  while (walk.next(&g)) {
-    const Shape shape = shape_of(a, g);
-    if (shape.blocks == 0) continue;
-    ok = ok && mbar_wait(&b->q_empty, (segment & 1) ^ 1, kSiteAttention);
+  while (true) {
+    const SegmentEntry e = *reader.wait();
+    reader.release();
+    if (!reader.ok || e.blocks < 0) return;
+    if (e.blocks == 0) continue;
+    bool ok = mbar_wait(&b->q_empty, (segment & 1) ^ 1, kSiteAttention);
     ++segment;
     if (!ok) return;
-    const int tiles = shape.pair ? 2 : 1;
+    const int tiles = e.pair != 0 ? 2 : 1;
     mbar_expect_tx(&b->q_full, tiles * S::kHalves * tokens * a.group * 128);
     for (int t = 0; t < tiles; ++t)
       for (int h = 0; h < S::kHalves; ++h)
-        tma_load_3d(smem + t * S::kTileBytes + h * S::kHalfBytes, &p.q, &b->q_full, h * 64, g.head * a.group,
-                    g.seq.q_row + (2 * g.unit + t) * tokens);
-    const auto block = [&](const CUtensorMap* map, int i) {
+        tma_load_3d(smem + t * S::kTileBytes + h * S::kHalfBytes, &p.q, &b->q_full, h * 64, e.head * a.group, e.q_row + t * tokens);
+    const CUtensorMap *k = &p.k[e.source], *v = &p.v[e.source];
+    for (int i = 0; i < 2 * e.blocks; ++i) {   // K and V of each block in turn
       const uint32_t slot = load % S::kSlots, round = load / S::kSlots;
       ++load;
-      ok = ok && mbar_wait(&b->empty[slot], (round & 1) ^ 1, kSiteAttention);
-      if (!ok) return;
-      mbar_expect_tx(&b->full[slot], S::kTileBytes);
+      if (!mbar_wait(&b->empty[slot], (round & 1) ^ 1, kSiteAttention)) return;
+      // Values with rows to be cleared arrive elsewhere first; who clears them signals `full`.
+      uint64_t* arrival = i + 1 == 2 * e.blocks && e.live_keys < kTile ? &b->raw[slot] : &b->full[slot];
+      mbar_expect_tx(arrival, S::kTileBytes);
       for (int h = 0; h < S::kHalves; ++h)
-        tma_load_4d(smem + (2 + slot) * S::kTileBytes + h * S::kHalfBytes, map, &b->full[slot], h * 64, g.head,
-                    g.seq.k_row + (g.block_begin + i) * kTile, g.seq.batch);
-    };
-    // In the order in which the MMAs will want them.
-    const CUtensorMap *k = &p.k[g.seq.source], *v = &p.v[g.seq.source];
-    const int ahead = shape.pair ? 1 : 2;
-    for (int i = 0; i < ahead && i < shape.blocks; ++i) block(k, i);
-    for (int i = 0; i < shape.blocks; ++i) {
-      block(v, i);
-      if (i + ahead < shape.blocks) block(k, i + ahead);
+        tma_load_4d(smem + (2 + slot) * S::kTileBytes + h * S::kHalfBytes, (i & 1) != 0 ? v : k, arrival, h * 64, e.head, e.k_row + (i >> 1) * kTile,
+                    e.batch);
     }
   }
 }
 
 // --------------------------------------------------------------------------------------- MMAs
 
+// One thread per stream.
 template <int kDim, bool kBf16>
-__device__ __forceinline__ void mma_role(const UmmaAttentionArgs& p, const WorkStart& start, uint8_t* smem, Shared* b, uint32_t tmem) {
+__device__ __forceinline__ void mma_role(const UmmaAttentionArgs& p, uint8_t* smem, Shared* b, uint32_t tmem, int s) {
   using S = Smem<kDim>;
   const AttentionArgs& a = p.a;
-  const int lane = threadIdx.x & 31;
-  const uint32_t idesc_s = umma_idesc_f16(kTile, kTile, kBf16, false, false);
+  constexpr uint32_t kIdescS = umma_idesc_f16(kTile, kTile, kBf16, false, false);
   const uint32_t idesc_o = umma_idesc_f16(kTile, (a.dim + 15) / 16 * 16, kBf16, false, true);
   const int steps = (a.dim + 15) / 16;   // of 16 along the head dimension; what lies behind it reads as zero
-  SegmentWalk<kUmmaKeyBlock> walk(a, start);
-  Segment g;
-  bool ok = true;
-  uint32_t load = 0, segment = 0, item[2] = {0, 0};
-  while (walk.next(&g)) {
-    const Shape shape = shape_of(a, g);
-    if (shape.blocks == 0) continue;
-    ok = ok && mbar_wait(&b->q_full, segment & 1, kSiteAttention);
-    uint32_t k_slot = 0, v_slot = 0;
-    const auto arrived = [&]() {   // the next block of the ring
-      const uint32_t slot = load % S::kSlots, round = load / S::kSlots;
-      ++load;
-      ok = ok && mbar_wait(&b->full[slot], round & 1, kSiteAttention);
-      return slot;
-    };
-    const int items = shape.items();
-    const auto block_of = [&](int j) { return shape.pair ? j / 2 : j; };
-    const auto first_use = [&](int j) { return !shape.pair || j % 2 == 0; };
-    const auto last_use = [&](int j) { return !shape.pair || j % 2 == 1; };
-    const auto scores = [&](int j) {
-      if (first_use(j)) k_slot = arrived();
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) return;
-      if (lane == 0) {
-        tcgen05_fence_after_sync();
-        const uint32_t q_at = smem_u32(smem) + (shape.pair ? (j & 1) * S::kTileBytes : 0);
-        const uint32_t k_at = smem_u32(smem) + (2 + k_slot) * S::kTileBytes;
-        const uint64_t qd = umma_smem_desc(q_at, 16, 1024, kUmmaSwizzle128B), kd = umma_smem_desc(k_at, 16, 1024, kUmmaSwizzle128B);
-        for (int step = 0; step < steps; ++step) {
-          const uint32_t at = (step >> 2) * S::kHalfBytes + (step & 3) * 32;
-          umma_f16(tmem + kColS + (j & 1) * kColStream, umma_desc_advance(qd, at), umma_desc_advance(kd, at), idesc_s, step > 0);
-        }
-        if (last_use(j)) umma_commit(&b->empty[k_slot]);
-        if (j + 1 == items) umma_commit(&b->q_empty);
-        umma_commit(&b->s_full[j & 1]);
-      }
-      __syncwarp();
-    };
-    for (int j = 0; j < 2 && j < items; ++j) scores(j);
-    for (int j = 0; j < items; ++j) {
-      const int s = j & 1;
-      if (first_use(j)) {
-        v_slot = arrived();
-        const int live = g.seq.m - (g.block_begin + block_of(j)) * kTile;
-        if (ok && live < kTile) {   // rows of other owners: zero, whatever they are
-          uint8_t* v = smem + (2 + v_slot) * S::kTileBytes;
-          for (int i = live * 8 + lane; i < kTile * 8; i += 32)
-            for (int h = 0; h < S::kHalves; ++h)
-              *reinterpret_cast<uint4*>(v + h * S::kHalfBytes + i * 16) = make_uint4(0, 0, 0, 0);
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
-      }
-      if (j == 0) ok = ok && mbar_wait(&b->o_empty, (segment & 1) ^ 1, kSiteAttention);
-      ok = ok && mbar_wait(&b->p_ready[s], item[s] & 1, kSiteAttention);
-      ++item[s];
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok && lane == 0) {
-        tcgen05_fence_after_sync();
-        const uint64_t vd = umma_smem_desc(smem_u32(smem) + (2 + v_slot) * S::kTileBytes, S::kHalfBytes, 1024, kUmmaSwizzle128B);
-        for (int step = 0; step < kTile / 16; ++step)
-          umma_f16_tmem_a(tmem + kColO + s * kColStream, tmem + kColS + s * kColStream + step * 8, umma_desc_advance(vd, step * 2048), idesc_o,
-                          j >= 2 || step > 0);
-        if (last_use(j)) umma_commit(&b->empty[v_slot]);
-        if (j + 1 == items) umma_commit(&b->o_full);
-      }
-      __syncwarp();
-      if (j + 2 < items) scores(j + 2);
-    }
+  const uint64_t q_desc[2] = {umma_smem_desc(smem_u32(smem), 16, 1024, kUmmaSwizzle128B),
+                              umma_smem_desc(smem_u32(smem) + S::kTileBytes, 16, 1024, kUmmaSwizzle128B)};
+  const uint64_t k_desc = umma_smem_desc(smem_u32(smem) + 2 * S::kTileBytes, 16, 1024, kUmmaSwizzle128B);
+  const uint64_t v_desc = umma_smem_desc(smem_u32(smem) + 2 * S::kTileBytes, S::kHalfBytes, 1024, kUmmaSwizzle128B);
+  const uint32_t s_at = tmem + kColS + s * kColStream, o_at = tmem + kColO + s * kColStream;
+  EntryReader reader{b};
+  uint32_t load = 0, segment = 0, item = 0, own_segment = 0;
+  while (true) {
+    const SegmentEntry* entry = reader.wait();
+    const int blocks = entry->blocks;
+    const bool pair = entry->pair != 0;
+    reader.release();
+    if (!reader.ok || blocks < 0) return;
+    if (blocks == 0) continue;
+    if (!mbar_wait(&b->q_full, segment & 1, kSiteAttention)) return;
     ++segment;
+    const int step_blocks = pair ? 1 : 2, first = pair ? 0 : s;
+    // Both streams' threads count for a block of the ring; the one of a block that the other stream
+    // does not touch counts for it too.
+    const auto release = [&](uint32_t slot) {
+      if (!pair) mbar_arrive_relaxed(&b->empty[slot]);
+      umma_commit(&b->empty[slot]);
+    };
+    const auto scores = [&](int block) {
+      const uint32_t at = load + 2 * block, slot = at % S::kSlots;
+      if (!mbar_wait(&b->full[slot], at / S::kSlots & 1, kSiteAttention)) return false;
+      tcgen05_fence_after_sync();
+      const uint64_t qd = q_desc[pair ? s : 0], kd = umma_desc_advance(k_desc, slot * S::kTileBytes);
+#pragma unroll
+      for (int step = 0; step < kDim / 16; ++step) {
+        if (step >= steps) break;
+        const uint32_t offset = (step >> 2) * S::kHalfBytes + (step & 3) * 32;
+        umma_f16(s_at, umma_desc_advance(qd, offset), umma_desc_advance(kd, offset), kIdescS, step > 0);
+      }
+      umma_commit(&b->s_full[s]);
+      release(slot);
+      if (block + step_blocks >= blocks) umma_commit(&b->q_empty);
+      return true;
+    };
+    if (first >= blocks) {   // nothing for this stream
+      mbar_arrive(&b->q_empty);
+    } else {
+      if (!scores(first)) return;
+      for (int block = first; block < blocks; block += step_blocks) {
+        const uint32_t at = load + 2 * block + 1, slot = at % S::kSlots;
+        if (!mbar_wait(&b->full[slot], at / S::kSlots & 1, kSiteAttention)) return;
+        if (block == first && !mbar_wait(&b->o_empty[s], (own_segment & 1) ^ 1, kSiteAttention)) return;
+        if (!mbar_wait(&b->p_ready[s], item & 1, kSiteAttention)) return;
+        ++item;
+        tcgen05_fence_after_sync();
+        const uint64_t vd = umma_desc_advance(v_desc, slot * S::kTileBytes);
+#pragma unroll
+        for (int step = 0; step < kTile / 16; ++step)
+          umma_f16_tmem_a(o_at, s_at + step * 8, umma_desc_advance(vd, step * 2048), idesc_o, block != first || step > 0);
+        const bool last = block + step_blocks >= blocks;
+        if (last) umma_commit(&b->o_full[s]);
+        else if (!scores(block + step_blocks)) return;
+        release(slot);
+      }
+      ++own_segment;
+    }
+    load += 2 * blocks;
   }
 }
 
@@ -243,12 +320,19 @@ __device__ __forceinline__ void softmax_block(uint32_t s_at, uint32_t o_at, int 
   for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_at + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&x[32 * c]));
   tmem_ld_wait();
   loaded(x);
-  float top[4] = {kMinusInf, kMinusInf, kMinusInf, kMinusInf};
+  if (kMasked) {
 #pragma unroll
-  for (int i = 0; i < kTile; ++i) {
-    if (kMasked && i >= seen) x[i] = kMinusInf;   // chosen, not added: the product may be NaN
-    top[i & 3] = fmaxf(top[i & 3], x[i]);
+    for (int i = 0; i < kTile; ++i)
+      if (i >= seen) x[i] = kMinusInf;   // chosen, not added: the product may be NaN
   }
+  float top[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+  for (int i = 4; i < kTile - 4; i += 8) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top[j] = max3(top[j], x[i + j], x[i + 4 + j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], x[kTile - 4 + j]);
   const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
   if (first) {
     row->m = m;
@@ -259,123 +343,172 @@ __device__ __forceinline__ void softmax_block(uint32_t s_at, uint32_t o_at, int 
       const float keep = grown ? exp2_fast(row->m - next) : 1.f;
       row->l *= keep;
       row->m = next;
-      for (int c = 0; c < chunks; ++c) {
-        float o[32];
-        load_columns(o_at + 32 * c, o);
+      for (int c = 0; c < 2 * chunks; ++c) {
+        float o[16];
+        tmem_ld_32x16(o_at + 16 * c, *reinterpret_cast<uint32_t(*)[16]>(&o));
+        tmem_ld_wait();
+        loaded(o);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] *= keep;
-        tmem_st_32x32(o_at + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&o));
+        for (int i = 0; i < 16; ++i) o[i] *= keep;
+        tmem_st_32x16(o_at + 16 * c, *reinterpret_cast<uint32_t(*)[16]>(&o));
       }
     }
   }
   const float base = row->m == kMinusInf ? 0.f : row->m;   // nothing seen yet: all terms are 2^(-inf)
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  const uint64_t scale2 = pack_f32x2(scale, scale), base2 = pack_f32x2(-base, -base);
+  uint64_t sum[2] = {0, 0};
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    uint32_t packed[32];
+  for (int part = 0; part < 4; ++part) {
+    uint32_t packed[16];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const float lo = exp2_fast(fmaf(x[64 * half + 2 * i], scale, -base)), hi = exp2_fast(fmaf(x[64 * half + 2 * i + 1], scale, -base));
-      sum[(2 * i) & 3] += lo, sum[(2 * i + 1) & 3] += hi;
+    for (int i = 0; i < 16; ++i) {
+      const float2 y = unpack_f32x2(fma_f32x2(pack_f32x2(x[32 * part + 2 * i], x[32 * part + 2 * i + 1]), scale2, base2));
+      const float lo = exp2_fast(y.x), hi = exp2_fast(y.y);
+      sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(lo, hi));
       packed[i] = pack<kBf16>(lo, hi);
     }
-    tmem_st_32x32(s_at + 32 * half, packed);
+    tmem_st_32x16(s_at + 16 * part, packed);
   }
-  row->l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  const float2 total = unpack_f32x2(add_f32x2(sum[0], sum[1]));
+  row->l += total.x + total.y;
   tmem_st_wait();
 }
 
-// 32 finished columns of a row.
+// Finished columns [column, column + 32) of a warp's 32 rows. Each thread holds its row's, and rows lie
+// far apart: stored from the registers, every instruction would touch 32 lines of memory, which the
+// load/store unit takes one per cycle (8600 cycles a unit). So they are turned through the warp's 4 KiB
+// of shared memory, in 16-byte pieces whose place is permuted by the row to keep the banks apart;
+// then 4 or 8 lanes store each row's piece of 64 (16-bit) or 128 bytes. at: element offset of the
+// lane's row, -1: not there.
 template <bool kBf16>
-__device__ __forceinline__ void store_columns(const AttentionArgs& a, int64_t row, int column, const float (&y)[32]) {
-  if (a.split != 0) {
-    float* out = a.partial_o + row * a.dim + column;
+__device__ __forceinline__ void store_columns(const AttentionArgs& a, bool partial, uint4* stage, int lane, int64_t at, int column,
+                                              const float (&y)[32]) {
+  const int pieces = partial ? 8 : 4;
+  if (partial) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 4)
-      if (column + i < a.dim) *reinterpret_cast<float4*>(out + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+    for (int i = 0; i < 8; ++i)
+      stage[lane * 8 + (i ^ (lane & 7))] = make_uint4(__float_as_uint(y[4 * i]), __float_as_uint(y[4 * i + 1]), __float_as_uint(y[4 * i + 2]),
+                                                      __float_as_uint(y[4 * i + 3]));
   } else {
-    uint16_t* out = static_cast<uint16_t*>(a.out) + row * a.dim + column;
 #pragma unroll
-    for (int i = 0; i < 32; i += 8)
-      if (column + i < a.dim)
-        *reinterpret_cast<uint4*>(out + i) = make_uint4(pack<kBf16>(y[i], y[i + 1]), pack<kBf16>(y[i + 2], y[i + 3]),
-                                                        pack<kBf16>(y[i + 4], y[i + 5]), pack<kBf16>(y[i + 6], y[i + 7]));
+    for (int i = 0; i < 4; ++i)
+      stage[lane * 8 + (i ^ (lane & 7))] = make_uint4(pack<kBf16>(y[8 * i], y[8 * i + 1]), pack<kBf16>(y[8 * i + 2], y[8 * i + 3]),
+                                                      pack<kBf16>(y[8 * i + 4], y[8 * i + 5]), pack<kBf16>(y[8 * i + 6], y[8 * i + 7]));
   }
+  __syncwarp();
+  const int piece = lane & (pieces - 1), width = partial ? 4 : 8;   // elements of a piece
+  const bool inside = column + piece * width < a.dim;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int row = (partial ? j * 4 : j * 8) + lane / pieces;
+    if (!partial && j >= 4) break;
+    const int64_t to = __shfl_sync(0xffffffffu, at, row);
+    const uint4 v = stage[row * 8 + (piece ^ (row & 7))];
+    if (to >= 0 && inside) {
+      if (partial) *reinterpret_cast<uint4*>(a.partial_o + to + column + piece * 4) = v;
+      else *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + to + column + piece * 8) = v;
+    }
+  }
+  __syncwarp();
 }
 
 template <bool kBf16>
-__device__ __forceinline__ void softmax_role(const UmmaAttentionArgs& p, const WorkStart& start, Shared* b, uint32_t tmem) {
+__device__ __forceinline__ void softmax_role(const UmmaAttentionArgs& p, Shared* b, uint8_t* staging, uint32_t tmem) {
   const AttentionArgs& a = p.a;
   const int s = threadIdx.x >> 7;                    // stream
   const int r = threadIdx.x & 127;                   // row of the tile, TMEM lane
   const int warp_row = r & ~31, lane = r & 31;
   const uint32_t lanes = static_cast<uint32_t>(warp_row) << 16;
   const uint32_t s_at = tmem + lanes + kColS + s * kColStream, o_at = tmem + lanes + kColO + s * kColStream;
-  const int tile_rows = a.unit_rows / 2;
+  const uint32_t other_o_at = tmem + lanes + kColO + (s ^ 1) * kColStream;
+  uint4* stage = reinterpret_cast<uint4*>(staging + (threadIdx.x >> 5) * 4096);
+  const int tile_rows = a.unit_rows / 2, tile_tokens = a.tokens / 2;
+  const int token_r = r / a.group, head_r = r - token_r * a.group, token_warp = warp_row / a.group;   // within the tile
   const int chunks = (a.dim + 31) / 32;
-  SegmentWalk<kUmmaKeyBlock> walk(a, start);
-  Segment g;
+  EntryReader reader{b};
   bool ok = true;
-  uint32_t segment = 0, item = 0;
-  while (walk.next(&g)) {
-    const Shape shape = shape_of(a, g);
-    const int64_t rows = static_cast<int64_t>(g.seq.n) * a.group;
-    const int64_t tile0 = static_cast<int64_t>(g.unit) * a.unit_rows + (shape.pair && s == 1 ? tile_rows : 0);
-    const int64_t flat = tile0 + r;
-    const bool live = r < tile_rows && flat < rows;
-    const bool warp_live = warp_row < tile_rows && tile0 + warp_row < rows;   // some row of the warp is there
+  uint32_t item = 0, o_count[2] = {0, 0}, met = 0;
+  // All eight warps; a bounded wait, which a plain barrier has not.
+  const auto meet = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&b->exchanged);
+    ok = __all_sync(0xffffffffu, ok && mbar_wait(&b->exchanged, met & 1, kSiteAttention));
+    ++met;
+  };
+  while (true) {
+    const SegmentEntry* entry = reader.wait();
+    ok = __all_sync(0xffffffffu, ok && reader.ok);
+    const int blocks = ok ? entry->blocks : -1;
+    const bool pair = entry->pair != 0, partial = entry->partial != 0;
+    const int keys = entry->keys, ahead = entry->ahead, tokens = entry->tokens;
+    const int token0 = pair && s == 1 ? tile_tokens : 0;   // of the tile within the unit
+    const int64_t out_row = static_cast<int64_t>(entry->q_row + token0 + token_r) * a.heads + entry->head * a.group + head_r;
+    int64_t at = out_row;
+    if (partial) {
+      at = entry->partial_row >= 0 ? entry->partial_row + (pair && s == 1 ? tile_rows : 0) + r
+                                   : static_cast<int64_t>(a.ctas) * a.unit_rows + entry->source * static_cast<int64_t>(a.q_rows) * a.heads + out_row;
+    }
+    __syncwarp();
+    if (lane == 0) reader.release();
+    else ++reader.count;
+    if (blocks < 0) return;
+    const bool live = r < tile_rows && token0 + token_r < tokens;
+    const bool warp_live = warp_row < tile_rows && token0 + token_warp < tokens;   // some row of the warp is there
+    const int items = pair ? blocks : (blocks + 1 - s) / 2;
     RowState row{kMinusInf, 0.f};
-    if (shape.blocks > 0) {
-      const int seen = live ? visible_keys(a, g.seq, static_cast<int>(flat / a.group)) : 0;
-      // All rows of the warp that are there see at least what its first row sees.
-      const int seen_by_all = warp_live ? visible_keys(a, g.seq, static_cast<int>((tile0 + warp_row) / a.group)) : 0;
-      const int items = shape.of_stream(s);
-      for (int i = 0; i < items; ++i) {
-        const int key0 = (g.block_begin + (shape.pair ? i : 2 * i + s)) * kTile;
-        ok = __all_sync(0xffffffffu, ok && mbar_wait(&b->s_full[s], item & 1, kSiteAttention));
-        ++item;
-        if (ok && warp_live) {
-          tcgen05_fence_after_sync();
-          if (key0 + kTile <= seen_by_all) softmax_block<kBf16, false>(s_at, o_at, chunks, 0, a.scale_log2, i == 0, &row);
-          else softmax_block<kBf16, true>(s_at, o_at, chunks, seen - key0, a.scale_log2, i == 0, &row);
-          tcgen05_fence_before_sync();
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&b->p_ready[s]);
+    const int seen = live ? clamp_int(ahead + token0 + token_r, 0, keys) : 0;
+    // All rows of the warp that are there see at least what its first row sees.
+    const int seen_by_all = clamp_int(ahead + token0 + token_warp, 0, keys);
+    for (int i = 0; i < items; ++i) {
+      const int key0 = (pair ? i : 2 * i + s) * kTile;
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(&b->s_full[s], item & 1, kSiteAttention));
+      ++item;
+      if (ok && warp_live) {
+        tcgen05_fence_after_sync();
+        if (key0 + kTile <= seen_by_all) softmax_block<kBf16, false>(s_at, o_at, chunks, 0, a.scale_log2, i == 0, &row);
+        else softmax_block<kBf16, true>(s_at, o_at, chunks, seen - key0, a.scale_log2, i == 0, &row);
+        tcgen05_fence_before_sync();
       }
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(&b->o_full, segment & 1, kSiteAttention));
-      ++segment;
-      tcgen05_fence_after_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b->p_ready[s]);
     }
     // Rows of one tile that two streams worked on: the same thread of both warp groups owns them, and
     // each finishes every other 32 columns.
+    const bool joined = !pair && blocks > 1;
     float mine = 1.f, other = 0.f, total = row.l, base = row.m;
-    const bool joined = !shape.pair && shape.blocks > 1;
     if (joined) {
       b->exchange[s][r] = make_float2(row.m, row.l);
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      meet();
       const float2 peer = b->exchange[s ^ 1][r];
       base = fmaxf(row.m, peer.x);
       const float zero = base == kMinusInf ? 0.f : base;
       mine = exp2_fast(row.m - zero), other = exp2_fast(peer.x - zero);
       total = row.l * mine + peer.y * other;
-      asm volatile("bar.sync 1, 256;" ::: "memory");   // read by all before the next segment writes
+      meet();   // read by all before the next segment writes
     }
-    if (ok && warp_live && (shape.pair || s == 0 || joined)) {
-      const int64_t at = live ? (a.split != 0 ? partial_row(a, g, flat) : output_row(a, g, flat)) : 0;
-      if (a.split != 0 && live && (shape.pair || s == 0)) a.partial_ml[at] = make_float2(base, total);
-      const float inv = a.split != 0 ? 1.f : (total == 0.f ? 0.f : 1.f / total);
+#pragma unroll
+    for (int stream = 0; stream < 2; ++stream) {
+      if ((pair || stream == 0 || joined) && blocks > 0) {   // the stream has an accumulator
+        if (stream == s || joined) ok = __all_sync(0xffffffffu, ok && mbar_wait(&b->o_full[stream], o_count[stream] & 1, kSiteAttention));
+        ++o_count[stream];
+      }
+    }
+    tcgen05_fence_after_sync();
+    if (ok && warp_live && (pair || s == 0 || joined)) {
+      if (partial && live && (pair || s == 0)) a.partial_ml[at] = make_float2(base, total);
+      const float inv = partial ? 1.f : (total == 0.f ? 0.f : 1.f / total);
       const float f0 = mine * inv, f1 = other * inv;
+      const int64_t element = live ? at * a.dim : -1;
       for (int c = joined ? s : 0; c < chunks; c += joined ? 2 : 1) {
         float y[32];
-        if (shape.blocks > 0) {
+        if (blocks > 0) {
           load_columns(o_at + 32 * c, y);
           // A row that saw nothing keeps its zeros whatever its accumulator holds.
 #pragma unroll
           for (int i = 0; i < 32; ++i) y[i] = total == 0.f ? 0.f : y[i] * f0;
           if (joined) {
             float z[32];
-            load_columns(tmem + lanes + kColO + (s ^ 1) * kColStream + 32 * c, z);
+            load_columns(other_o_at + 32 * c, z);
 #pragma unroll
             for (int i = 0; i < 32; ++i) y[i] = total == 0.f ? 0.f : y[i] + z[i] * f1;
           }
@@ -383,13 +516,14 @@ __device__ __forceinline__ void softmax_role(const UmmaAttentionArgs& p, const W
 #pragma unroll
           for (int i = 0; i < 32; ++i) y[i] = 0.f;
         }
-        if (live) store_columns<kBf16>(a, at, 32 * c, y);
+        store_columns<kBf16>(a, partial, stage, lane, element, 32 * c, y);
       }
     }
-    if (shape.blocks > 0) {
-      tcgen05_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&b->o_empty);
+    tcgen05_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) {   // eight arrivals free an accumulator
+      if (joined) mbar_arrive(&b->o_empty[0]), mbar_arrive(&b->o_empty[1]);
+      else if (items > 0) mbar_arrive(&b->o_empty[s]), mbar_arrive(&b->o_empty[s]);
     }
   }
 }
@@ -398,34 +532,43 @@ template <int kDim, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1) attention_umma_kernel(const __grid_constant__ UmmaAttentionArgs p) {
   using S = Smem<kDim>;
   extern __shared__ __align__(1024) uint8_t smem[];   // the swizzle's period
-  Shared& bars = *reinterpret_cast<Shared*>(smem + S::kTiles);
+  Shared& b = *reinterpret_cast<Shared*>(smem + S::kTiles);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    prefetch_tensormap(&p.q);
-    for (int s = 0; s < S::kSlots; ++s) mbar_init(&bars.full[s], 1), mbar_init(&bars.empty[s], 1);
-    mbar_init(&bars.q_full, 1), mbar_init(&bars.q_empty, 1);
-    for (int s = 0; s < 2; ++s) mbar_init(&bars.s_full[s], 1), mbar_init(&bars.p_ready[s], 4);
-    mbar_init(&bars.o_full, 1), mbar_init(&bars.o_empty, 8);
+    for (int i = 0; i < S::kSlots; ++i) mbar_init(&b.full[i], 1), mbar_init(&b.empty[i], 2), mbar_init(&b.raw[i], 1);
+    for (int i = 0; i < kEntries; ++i) mbar_init(&b.entry_full[i], 1), mbar_init(&b.entry_empty[i], kEntryReaders);
+    mbar_init(&b.q_full, 1), mbar_init(&b.q_empty, 2), mbar_init(&b.exchanged, 8);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&b.s_full[s], 1), mbar_init(&b.p_ready[s], 4);
+      mbar_init(&b.o_full[s], 1), mbar_init(&b.o_empty[s], 8);
+    }
     mbar_init_fence();
   }
+  if (threadIdx.x == 256) {
+    prefetch_tensormap(&p.q);
+    for (int i = 0; i < (p.a.kind == kShared ? 2 : 1); ++i) prefetch_tensormap(&p.k[i]), prefetch_tensormap(&p.v[i]);
+  }
   if (warp == 9) {
-    tmem_alloc<512>(&bars.tmem);
+    tmem_alloc<512>(&b.tmem);
     tmem_relinquish();
   }
   tcgen05_fence_before_sync();
   __syncthreads();
   tcgen05_fence_after_sync();
-  const uint32_t tmem = bars.tmem;
+  const uint32_t tmem = b.tmem;
   grid_launch_dependents();   // after the allocation: a following kernel may want tensor memory too
   grid_dependency_wait();
-  const WorkStart start = find_attention_work<kUmmaKeyBlock, kThreads>(p.a, &bars.scratch);
+  const WorkStart start = find_range<kUmmaKeyBlock, kThreads>(p.a, &b.scratch, blockIdx.x);
   if (warp < 8) {
-    softmax_role<kBf16>(p, start, &bars, tmem);
-  } else if (warp == 8) {
-    if (lane == 0) copy_role<kDim>(p, start, smem, &bars);
+    registers_raise<kSoftmaxRegisters>();
+    softmax_role<kBf16>(p, &b, smem + S::kStaging, tmem);
   } else {
-    mma_role<kDim, kBf16>(p, start, smem, &bars, tmem);
+    registers_lower<kOtherRegisters>();
+    if (warp == 8 && lane == 0) copy_role<kDim>(p, smem, &b);
+    if ((warp == 9 || warp == 10) && lane == 0) mma_role<kDim, kBf16>(p, smem, &b, tmem, warp - 9);
+    if (warp == 11) segment_role<kDim>(p, start, smem, &b);
   }
+  __syncwarp();
   tcgen05_fence_before_sync();
   __syncthreads();
   tcgen05_fence_after_sync();
@@ -433,12 +576,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_umma_kernel(const __gri
 }
 
 template <int kDim, bool kBf16>
-int launch(const UmmaAttentionArgs& p, int64_t blocks, cudaStream_t s) {
+int launch(const UmmaAttentionArgs& p, cudaStream_t s) {
   constexpr size_t kBytes = Smem<kDim>::kTiles + sizeof(Shared);
   static_assert(kBytes <= 227 * 1024, "shared memory of one CTA");
   if (!ensure_dynamic_smem<attention_umma_kernel<kDim, kBf16>, kBytes>()) return B200_ERR_LAUNCH_FAILED;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.gridDim = dim3(static_cast<unsigned>(p.a.ctas));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kBytes;
   cfg.stream = s;
@@ -465,13 +608,12 @@ bool make_key_map(CUtensorMap* out, const void* base, const AttentionArgs& a, in
 
 void plan_attention_umma(AttentionArgs* a, int sms) {
   // Tiles hold whole tokens: a copy brings (dim, group, tokens) boxes.
-  a->unit_rows = 2 * (kTile / a->group) * a->group;
+  a->tokens = 2 * (kTile / a->group);
+  a->unit_rows = a->tokens * a->group;
   a->ctas = sms;
 }
 
-int launch_attention_umma(const AttentionArgs& a, cudaStream_t s, int64_t units) {
-  const int64_t blocks = a.split != 0 ? a.ctas : units * a.kv_heads;
-  if (blocks > 0x7fffffffLL) return B200_ERR_INVALID_PROBLEM;
+int launch_attention_umma(const AttentionArgs& a, cudaStream_t s) {
   UmmaAttentionArgs p;
   p.a = a;
   const bool bf16 = a.dtype == B200_BF16;
@@ -492,8 +634,8 @@ int launch_attention_umma(const AttentionArgs& a, cudaStream_t s, int64_t units)
     }
   }
   if (!ok) return B200_ERR_INVALID_PROBLEM;
-  if (a.dim <= 64) return bf16 ? launch<64, true>(p, blocks, s) : launch<64, false>(p, blocks, s);
-  return bf16 ? launch<128, true>(p, blocks, s) : launch<128, false>(p, blocks, s);
+  if (a.dim <= 64) return bf16 ? launch<64, true>(p, s) : launch<64, false>(p, s);
+  return bf16 ? launch<128, true>(p, s) : launch<128, false>(p, s);
 }
 
 }  // namespace b200

@@ -94,7 +94,7 @@ torch::Tensor attention_prompt(const torch::Tensor& q_in, const torch::Tensor& k
   const auto cu_k = cu_k_in.has_value() ? int32_vector(*cu_k_in, "cu_seqlens_k", q_in, "q") : cu_q;
   TORCH_CHECK(cu_q.size(0) >= 1 && cu_k.size(0) == cu_q.size(0), "cu_seqlens_q and cu_seqlens_k must hold one more offset than there are sequences");
   TORCH_CHECK(cu_k_in.has_value() || k_in.size(0) == q_in.size(0), "cu_seqlens_k is required when k has other rows than q");
-  check_limit(q_in.size(0), "q");
+  check_limit(q_in.size(0) * (q_in.size(1) / k_in.size(1)), "q");
   check_limit(k_in.size(0), "k");
   const c10::cuda::CUDAGuard guard(q_in.device());
   const auto q = granular(q_in), k = granular(k_in), v = granular(v_in);
@@ -110,8 +110,9 @@ torch::Tensor attention_prompt(const torch::Tensor& q_in, const torch::Tensor& k
   p.scale = scale_or_default(scale, q.size(2));
   p.causal = causal;
   const size_t bytes = b200_attention_prompt_workspace_bytes(&p);
-  const auto workspace = torch::empty({static_cast<int64_t>(bytes)}, q.options().dtype(torch::kUInt8));
-  check_status(b200_attention_prompt(&p, workspace.data_ptr(), bytes, current_stream(q)), "attention_prompt");
+  torch::Tensor workspace;
+  if (bytes > 0) workspace = torch::empty({static_cast<int64_t>(bytes)}, q.options().dtype(torch::kUInt8));
+  check_status(b200_attention_prompt(&p, bytes > 0 ? workspace.data_ptr() : nullptr, bytes, current_stream(q)), "attention_prompt");
   return out;
 }
 
@@ -132,7 +133,7 @@ torch::Tensor attention_shared_prefix(const torch::Tensor& q_in, const torch::Te
   check_heads(q_in, kv_heads);
   const auto lengths = int32_vector(lengths_in, "lengths", q_in, "q");
   TORCH_CHECK(lengths.size(0) == batch, "lengths must have one entry per request");
-  check_limit(batch, "q");
+  check_limit(batch * (q_in.size(1) / kv_heads), "q");
   check_limit(k_prefix_in.size(0), "k_prefix");
   check_limit(k_cache_in.size(1), "k_cache");
   const c10::cuda::CUDAGuard guard(q_in.device());
