@@ -20,95 +20,100 @@ __device__ __forceinline__ void store_row4(void* out, int dtype, int64_t at, flo
   }
 }
 
-// Joins the partial results c of one row, a warp per row, in CTA order:
-// O = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c. One with l = 0 saw no key; its O is not read.
+// O = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over the partial results c of a row, in CTA order.
+// One with l = 0 saw no key; its O is not used. A CTA joins eight rows: lane (r, q) of warp w holds
+// columns 4 (4 k + q) .. + 3, k = w and w + 4, of row r, so that slots are read and rows written in whole
+// sectors, and up to four partial results of a row are on their way at a time.
 struct RowJoin {
+  const AttentionArgs& a;
+  int quad[2];   // of four columns
   float top = kMinusInf, total = 0.f;
-  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 sum[2];
 
-  __device__ __forceinline__ void add(const AttentionArgs& a, int64_t at, int lane) {
-    const float2 ml = a.partial_ml[at];
-    if (ml.y == 0.f) return;
-    const float next = fmaxf(top, ml.x);
+  __device__ __forceinline__ explicit RowJoin(const AttentionArgs& args) : a(args) {
+    quad[0] = (threadIdx.x >> 5) * 4 + (threadIdx.x & 31) / 8, quad[1] = quad[0] + 16;
+    sum[0] = sum[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  struct Part {
+    float2 ml;
+    float4 o[2];
+  };
+  __device__ __forceinline__ Part load(int64_t slot, int pitch, int row) const {
+    Part p;
+    p.ml = a.partial_ml[slot + row];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      p.o[i] = quad[i] * 4 < a.dim ? *reinterpret_cast<const float4*>(a.partial_o + slot * a.dim + (static_cast<int64_t>(quad[i]) * pitch + row) * 4)
+                                   : make_float4(0.f, 0.f, 0.f, 0.f);
+    return p;
+  }
+  __device__ __forceinline__ void add(const Part& p) {
+    if (p.ml.y == 0.f) return;
+    const float next = fmaxf(top, p.ml.x);
     const float base = next == kMinusInf ? 0.f : next;   // maxima of -infinity with l != 0: NaN rows
-    const float keep = exp2f(top - base), more = exp2f(ml.x - base);
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (lane * 4 < a.dim) v = *reinterpret_cast<const float4*>(a.partial_o + at * a.dim + lane * 4);
-    sum = make_float4(sum.x * keep + v.x * more, sum.y * keep + v.y * more, sum.z * keep + v.z * more, sum.w * keep + v.w * more);
-    total = total * keep + ml.y * more;
+    const float keep = exp2f(top - base), more = exp2f(p.ml.x - base);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      sum[i] = make_float4(sum[i].x * keep + p.o[i].x * more, sum[i].y * keep + p.o[i].y * more, sum[i].z * keep + p.o[i].z * more,
+                           sum[i].w * keep + p.o[i].w * more);
+    total = total * keep + p.ml.y * more;
     top = next;
   }
-  __device__ __forceinline__ void store(const AttentionArgs& a, int64_t row, int lane) const {
+  // The opened slot, then the continued ones of CTAs first + 1 .. last.
+  __device__ __forceinline__ void unit(int64_t slot, int pitch, int row, int first, int last) {
+    add(load(slot, pitch, row));
+    int c = first + 1;
+    for (; c + 3 <= last; c += 4) {
+      Part p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = load(continued_slot(a, c + i), a.unit_rows, row);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) add(p[i]);
+    }
+    for (; c <= last; ++c) add(load(continued_slot(a, c), a.unit_rows, row));
+  }
+  __device__ __forceinline__ void store(int64_t row) const {
     const float inv = total == 0.f ? 0.f : 1.f / total;
-    if (lane * 4 < a.dim) store_row4(a.out, a.dtype, row * a.dim + lane * 4, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (quad[i] * 4 < a.dim)
+        store_row4(a.out, a.dtype, row * a.dim + quad[i] * 4, make_float4(sum[i].x * inv, sum[i].y * inv, sum[i].z * inv, sum[i].w * inv));
   }
 };
+static_assert(kJoinWarps == 4, "columns of a row over the warps of a CTA");
 
-// Prompt calls: block (c, y) handles rows y, y + gridDim.y, ... (in groups of a warp each) of the unit
-// that boundary c cuts, if c is the first that does.
-template <int kKeys>
+// Prompt calls: block (c, y) handles rows 8 y .. 8 y + 7 of the unit that CTA c left open.
 __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_cuts_kernel(const AttentionArgs a) {
-  __shared__ WorkScratch scratch;
   grid_launch_dependents();
   grid_dependency_wait();
-  const int cta = blockIdx.x + 1;
-  const WorkStart start = find_range<kKeys, kJoinWarps * 32>(a, &scratch, cta);
-  if (start.sequence < 0 || start.block == 0 || start.before / start.per != cta - 1) return;
-  const Sequence seq = sequence_of(a, start.sequence);
-  const int last = static_cast<int>((start.before + unit_weight<kKeys>(a, seq, start.unit) - 1) / start.per);
-  const int row0 = start.unit * a.unit_rows;
-  const int rows = min(a.unit_rows, seq.n * a.group - row0);
-  const int lane = threadIdx.x & 31;
-  for (int r = blockIdx.y * kJoinWarps + (threadIdx.x >> 5); r < rows; r += gridDim.y * kJoinWarps) {
-    RowJoin join;
-    const int64_t out = output_row(a, seq, start.head, row0 + r);
-    join.add(a, opened_row(a, seq, out, cta - 1, r), lane);
-    for (int c = cta; c <= last; ++c) join.add(a, continued_row(a, c, r), lane);
-    join.store(a, out, lane);
-  }
+  const CutRecord cut = a.cuts[blockIdx.x];
+  const int row = blockIdx.y * 8 + (threadIdx.x & 7);
+  if (row >= cut.rows) return;
+  RowJoin join(a);
+  join.unit(continued_slot(a, a.ctas + blockIdx.x), a.unit_rows, row, cut.first, cut.last);
+  join.store(output_row(a, cut.q_row, cut.head, cut.row0 + row));
 }
 
-// Shared-prefix calls: a warp per row, which has a part over the prefix and one over its own keys. All
-// rows of a block belong to one request (blockIdx.x); the block finds the requests' first blocks by
-// itself.
-template <int kKeys>
+// Shared-prefix calls: block (x, h) handles rows 8 x .. 8 x + 7 of key head h: their part over the
+// prefix, and the one over their request's own keys.
 __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_rows_kernel(const AttentionArgs a) {
-  __shared__ int64_t sums[2][kJoinWarps];
   grid_launch_dependents();
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31, request = blockIdx.x;
-  const auto head_size = [&](int s) { return head_weight<kKeys>(a, sequence_of(a, s)); };
-  int64_t all = 0, before = 0;   // blocks of a key head: of all sequences, and of those ahead of this request
-  for (int s = threadIdx.x; s < a.sequences; s += kJoinWarps * 32) {
-    const int64_t size = head_size(s);
-    all += size;
-    if (s < request + 1) before += size;
+  const int flat = blockIdx.x * 8 + (threadIdx.x & 7), head = blockIdx.y;
+  if (flat >= a.q_rows * a.group) return;
+  const int request = flat / a.group, g = flat - request * a.group;
+  RowJoin join(a);
+  if (a.k_rows > 0) {
+    const int unit = flat / a.unit_rows;
+    const CutRecord cut = a.cuts[prefix_record(a, unit, head)];
+    join.unit(prefix_slot(a, unit, head), a.unit_rows, flat - unit * a.unit_rows, cut.first, cut.last);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o), before += __shfl_xor_sync(0xffffffffu, before, o);
-  if (lane == 0) sums[0][threadIdx.x >> 5] = all, sums[1][threadIdx.x >> 5] = before;
-  __syncthreads();
-  all = before = 0;
-  for (int w = 0; w < kJoinWarps; ++w) all += sums[0][w], before += sums[1][w];
-  const int64_t per = quotient(a.kv_heads * all + a.ctas - 1, a.ctas);
-  const Sequence prefix = sequence_of(a, 0), own = sequence_of(a, 1 + request);
-  for (int h = blockIdx.y * kJoinWarps + (threadIdx.x >> 5); h < a.heads; h += gridDim.y * kJoinWarps) {
-    const int head = h / a.group, g = h - head * a.group;
-    RowJoin join;
-    const int64_t out = static_cast<int64_t>(request) * a.heads + h;
-    const auto part = [&](const Sequence& seq, int64_t first_of_sequence, int flat) {
-      const int unit = flat / a.unit_rows, row = flat - unit * a.unit_rows;
-      const int blocks = unit_blocks<kKeys>(a, seq, unit);
-      if (blocks == 0) return;
-      const int64_t first = first_of_sequence + head * head_weight<kKeys>(a, seq) + weight_before<kKeys>(a, seq, unit);
-      const int c0 = static_cast<int>(quotient(first, per)), c1 = static_cast<int>(quotient(first + blocks - 1, per));
-      join.add(a, opened_row(a, seq, out, c0, row), lane);
-      for (int c = c0 + 1; c <= c1; ++c) join.add(a, continued_row(a, c, row), lane);
-    };
-    part(prefix, 0, request * a.group + g);
-    part(own, a.kv_heads * before, g);
-    join.store(a, out, lane);
+  if (sequence_of(a, 1 + request).m > 0) {
+    const int unit = g / a.unit_rows;
+    const CutRecord cut = a.cuts[own_record(a, request, head, unit)];
+    join.unit(own_slot(a, request, head, unit), own_pitch(a, unit), g - unit * a.unit_rows, cut.first, cut.last);
   }
+  join.store(static_cast<int64_t>(request) * a.heads + head * a.group + g);
 }
 
 // FP32 operands would lose half their bits on the tensor cores; 16-bit ones lose nothing.
@@ -127,13 +132,10 @@ int launch_join(Kernel kernel, dim3 grid, const AttentionArgs& a, cudaStream_t s
   return launch_status();
 }
 
-template <int kKeys>
 int join(const AttentionArgs& a, cudaStream_t s) {
-  if (a.kind == kShared) {
-    const unsigned share = static_cast<unsigned>((a.heads + kJoinWarps - 1) / kJoinWarps);
-    return launch_join(attention_join_rows_kernel<kKeys>, dim3(static_cast<unsigned>(a.q_rows), share < 32 ? share : 32), a, s);
-  }
-  return a.ctas < 2 ? B200_OK : launch_join(attention_join_cuts_kernel<kKeys>, dim3(static_cast<unsigned>(a.ctas) - 1, 8), a, s);
+  if (a.kind == kShared)
+    return launch_join(attention_join_rows_kernel, dim3(static_cast<unsigned>((a.q_rows * static_cast<int64_t>(a.group) + 7) / 8), a.kv_heads), a, s);
+  return launch_join(attention_join_cuts_kernel, dim3(static_cast<unsigned>(a.ctas), (a.unit_rows + 7) / 8), a, s);
 }
 
 // ------------------------------------------------------------------- arguments
@@ -200,60 +202,81 @@ int make_args(const b200_attention_shared_problem& q, AttentionArgs* a) {
   return B200_OK;
 }
 
-// Decomposition, without the lengths: returns whether there may be partial results.
-bool plan(AttentionArgs* a) {
+// Decomposition, as far as it does not depend on the lengths.
+struct Plan {
+  int status;
+  bool partial;   // there may be partial results
+};
+Plan plan(AttentionArgs* a) {
   const int sms = sm_count() > 0 ? sm_count() : 1;
   on_tensor_cores(*a) ? plan_attention_umma(a, sms) : plan_attention_simt(a, sms);
   a->token_shift = log2_or_minus_one(a->tokens);
   const int64_t keys = on_tensor_cores(*a) ? kUmmaKeyBlock : kSimtKeyBlock;
   const auto blocks = [&](int64_t rows) { return (rows + keys - 1) / keys; };
+  const auto units = [&](int64_t rows) { return (rows + a->unit_rows - 1) / a->unit_rows; };
+  const int64_t longest = blocks(a->k_rows);
+  int64_t most;        // length of the line
+  int64_t ranges;      // more CTAs than this would have nothing to do
   if (a->kind == kShared) {
-    // Never more ranges than blocks.
-    const int64_t own = (a->group + a->unit_rows - 1) / a->unit_rows * static_cast<int64_t>(a->q_rows) * blocks(a->room);
-    const int64_t prefix = (static_cast<int64_t>(a->q_rows) * a->group + a->unit_rows - 1) / a->unit_rows * blocks(a->k_rows);
-    const int64_t most = (own + prefix) * a->kv_heads;
-    if (most < a->ctas) a->ctas = static_cast<int>(most > 0 ? most : 1);
-    return true;
+    if (a->kv_heads > 65535) return {B200_ERR_INVALID_PROBLEM, false};   // a dimension of the join's grid
+    const int64_t prefix = units(static_cast<int64_t>(a->q_rows) * a->group), own = units(a->group) * a->q_rows;
+    ranges = (prefix * longest + own * blocks(a->room)) * a->kv_heads;
+    most = ranges + (prefix + own) * a->kv_heads * a->unit_cost;
+  } else {
+    // Each sequence, and the rows behind them, rounds up once.
+    const int64_t all = (static_cast<int64_t>(a->q_rows) * a->group / a->unit_rows + a->sequences + 1) * a->kv_heads;
+    ranges = all * (longest > 0 ? longest : 1);
+    most = all * (longest + a->unit_cost);
   }
-  // Each sequence, and the rows behind them, rounds up once.
-  const int64_t units = (static_cast<int64_t>(a->q_rows) * a->group / a->unit_rows + a->sequences + 1) * a->kv_heads;
-  const int64_t longest = blocks(a->k_rows) > 0 ? blocks(a->k_rows) : 1;
-  if (units < a->ctas && units * longest < a->ctas) a->ctas = static_cast<int>(units * longest);
-  return longest > 1;   // units of one block are never cut
+  // On the device the line is counted in 32 bits; it would take minutes to work through.
+  if (most > 0x7fffffff) return {B200_ERR_INVALID_PROBLEM, false};
+  if (ranges < a->ctas) a->ctas = static_cast<int>(ranges > 0 ? ranges : 1);
+  return {B200_OK, a->kind == kShared || longest > 1};   // units of one block are never cut
 }
 
 struct Workspace {
-  size_t o, total;   // maxima and denominators first
+  size_t cuts, o, total;   // maxima and denominators first
 };
 Workspace workspace_of(const AttentionArgs& a) {
   const auto round = [](size_t v) { return (v + 255) & ~size_t{255}; };
-  const size_t cuts = static_cast<size_t>(a.ctas) * a.unit_rows;
-  const size_t rows = cuts + (a.kind == kShared ? 2 * static_cast<size_t>(a.q_rows) * a.heads : cuts);
+  const auto units = [&](size_t rows) { return (rows + a.unit_rows - 1) / a.unit_rows; };
+  size_t rows = static_cast<size_t>(a.ctas) * a.unit_rows, records = a.ctas;
+  if (a.kind == kPrompt) {
+    rows *= 2;
+  } else {
+    const size_t prefix = units(static_cast<size_t>(a.q_rows) * a.group) * a.kv_heads;
+    rows += prefix * a.unit_rows + static_cast<size_t>(a.q_rows) * a.heads;
+    records = prefix + static_cast<size_t>(a.q_rows) * a.kv_heads * units(a.group);
+  }
   Workspace w{};
-  w.o = round(rows * sizeof(float2));
+  w.cuts = round(rows * sizeof(float2));
+  w.o = w.cuts + round(records * sizeof(CutRecord));
   w.total = w.o + round(rows * a.dim * sizeof(float));
   return w;
 }
 
 int run(AttentionArgs& a, void* workspace, size_t bytes, cudaStream_t s) {
-  const bool partial = plan(&a);
-  if (partial) {
+  const Plan planned = plan(&a);
+  if (planned.status != B200_OK) return planned.status;
+  if (planned.partial) {
     const Workspace w = workspace_of(a);
     if (workspace == nullptr || bytes < w.total) return B200_ERR_INVALID_ARGUMENT;
     if (!aligned16(workspace)) return B200_ERR_MISALIGNED_OPERAND;
-    a.partial_ml = static_cast<float2*>(workspace);
-    a.partial_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + w.o);
+    uint8_t* base = static_cast<uint8_t*>(workspace);
+    a.partial_ml = reinterpret_cast<float2*>(base);
+    a.cuts = reinterpret_cast<CutRecord*>(base + w.cuts);
+    a.partial_o = reinterpret_cast<float*>(base + w.o);
   }
   const int rc = on_tensor_cores(a) ? launch_attention_umma(a, s) : launch_attention_simt(a, s);
-  if (rc != B200_OK || !partial) return rc;
-  return on_tensor_cores(a) ? join<kUmmaKeyBlock>(a, s) : join<kSimtKeyBlock>(a, s);
+  return rc != B200_OK || !planned.partial ? rc : join(a, s);
 }
 
 template <class Problem>
 size_t workspace_bytes(const Problem* problem) {
   AttentionArgs a;
   if (problem == nullptr || make_args(*problem, &a) != B200_OK) return 0;
-  return plan(&a) ? workspace_of(a).total : 0;
+  const Plan planned = plan(&a);
+  return planned.status == B200_OK && planned.partial ? workspace_of(a).total : 0;
 }
 
 }  // namespace

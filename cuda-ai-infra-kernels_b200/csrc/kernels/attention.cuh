@@ -9,14 +9,14 @@
 // is: a decoding batch fills a tile with requests and heads as a prompt fills it with tokens.
 //
 // A unit is `unit_rows` such rows of one key head; its keys are cut in blocks, 128 or 64 keys each. All
-// blocks of all units, in the order sequence, head, unit, block, are dealt out in equal contiguous
+// units, in the order sequence, head, unit, are laid end to end, each as long as its blocks plus
+// `unit_cost` for what a unit costs beside them, and the line is dealt out in equal contiguous
 // ranges, one per CTA, whatever the lengths are. (One CTA per unit, longest first, left the tensor
 // pipe idle at the start and end of every unit and the machine uneven at the end of a call.) A unit
 // that lies inside one range is finished by its CTA. One that is cut by a range boundary leaves one
 // partial result (sum, maximum, denominator) per CTA that worked on it, and a second launch joins
 // them in CTA order: at most one unit per boundary, so the traffic does not grow with the call. In a
 // shared-prefix call every row has two units, one per part of its keys, and all results are partial.
-// In a prompt call a unit that sees no key counts as one block, so that somebody writes its zeros.
 // Lengths are read on the device only. Offsets and lengths are clamped to the arrays here.
 #pragma once
 
@@ -47,12 +47,23 @@ struct AttentionArgs {
   int unit_rows;
   int tokens;                        // of a unit; 0 where a group is larger than a unit, and units cut tokens
   int token_shift;                   // its logarithm where it is a power of two, else -1
+  int unit_cost;
   int ctas;                          // ranges
-  // Partial results: [row][dim], not divided by the denominator. First come the rows of units that
-  // are continued from the CTA before (unit_rows for each CTA), then those of units that are opened:
-  // unit_rows for each CTA in a prompt call, (part, output row) in a shared-prefix call.
+  // Partial results, in slots of some rows: maximum (scaled, base 2) and denominator [row], and the sum,
+  // not divided by it, as [dim / 4][row][4], so that the threads of a warp, which own one row
+  // each, write and read whole lines. First the slots of units continued from the CTA before,
+  // one of unit_rows rows per CTA, then those of units that a CTA opens: one per CTA in a prompt call;
+  // in a shared-prefix call one per prefix unit and head, and then `group` rows per request and head.
   float* partial_o;
-  float2* partial_ml;                // maximum (scaled, base 2), denominator
+  float2* partial_ml;
+  struct CutRecord* cuts;            // of each CTA in a prompt call, of each unit in a shared-prefix call
+};
+
+// What the join has to know about an opened unit; written by the CTA that opens it.
+struct CutRecord {
+  int first, last;         // CTAs that worked on it
+  int rows;                // prompt: 0 where the CTA left no unit open
+  int q_row, head, row0;   // prompt: the sequence's first query row, the key head, the unit's first row
 };
 
 struct Sequence {
@@ -110,151 +121,152 @@ __device__ __forceinline__ int unit_blocks(const AttentionArgs& a, const Sequenc
   return (visible_keys(a, s, min(last, s.n - 1)) + kKeys - 1) / kKeys;
 }
 
-// What a unit counts in the ranges.
-template <int kKeys>
-__device__ __forceinline__ int unit_weight(const AttentionArgs& a, const Sequence& s, int unit) {
-  const int blocks = unit_blocks<kKeys>(a, s, unit);
-  return blocks == 0 && a.kind == kPrompt ? 1 : blocks;
-}
-
-// Quotient of numbers that are small as a rule: a 64-bit division costs a hundred instructions.
-__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
-  if (((x | y) >> 32) == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(y);
-  return x / y;
+// Length of a unit on the line. A prompt's unit that sees no key is there all the same: somebody has
+// to write its zeros.
+__device__ __forceinline__ int unit_length(const AttentionArgs& a, int blocks) {
+  return blocks > 0 || a.kind == kPrompt ? blocks + a.unit_cost : 0;
 }
 
 // sum over i = 0 .. n - 1 of floor((a i + b) / m), for a, b >= 0: the whole multiples of m in a and b
 // come out as closed sums; what is left counts lattice points under a line, and counting them by
 // the other coordinate is the same sum with a and m exchanged, as in Euclid's algorithm.
-__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+static __device__ __noinline__ int64_t floor_sum(int n, int m, int a, int b) {
   int64_t sum = 0;
   while (n > 0) {
-    const int64_t whole_a = quotient(a, m), whole_b = quotient(b, m);
-    sum += n * (n - 1) / 2 * whole_a + n * whole_b;
+    const int whole_a = a / m, whole_b = b / m;
+    sum += static_cast<int64_t>(n) * (n - 1) / 2 * whole_a + static_cast<int64_t>(n) * whole_b;
     a -= whole_a * m, b -= whole_b * m;
-    const int64_t top = a * n + b;
+    const int64_t top = static_cast<int64_t>(a) * n + b;
     if (top < m) break;
-    n = quotient(top, m), b = top - n * m;
-    const int64_t t = m;
+    n = static_cast<int>(top / m), b = static_cast<int>(top - static_cast<int64_t>(n) * m);
+    const int t = m;
     m = a, a = t;
   }
   return sum;
 }
 
-// Weight of the first `units` units of one key head of the sequence.
+// Length of the first `units` of the `all` units of one key head of the sequence. The launcher has made
+// sure that the whole line fits 32 bits.
 template <int kKeys>
-__device__ __noinline__ int64_t weight_before(const AttentionArgs& a, const Sequence& s, int units) {
+__device__ __forceinline__ int length_before(const AttentionArgs& a, const Sequence& s, int units, int all) {
   if (units == 0) return 0;
-  if (a.kind == kShared || a.causal == 0) return static_cast<int64_t>(units) * unit_weight<kKeys>(a, s, 0);
+  if (a.kind == kShared || a.causal == 0) return units * unit_length(a, unit_blocks<kKeys>(a, s, 0));
   if (a.tokens == 0) {
-    int64_t sum = 0;
-    for (int t = 0; t < units; ++t) sum += unit_weight<kKeys>(a, s, t);
+    int sum = 0;
+    for (int t = 0; t < units; ++t) sum += unit_length(a, unit_blocks<kKeys>(a, s, t));
     return sum;
   }
   // Unit t holds whole tokens; but for the last of all, its last token sees c + tokens * (t + 1) keys.
-  // Where tokens is a power of two that divides the block, t advances the quotient by one every
-  // 2^shift units, and where it is a multiple of the block by a constant: no division.
-  const int tokens = a.tokens, all = unit_count(a, s);
-  const int64_t c = static_cast<int64_t>(s.m) - s.n;
-  const int64_t regular = units < all ? units : all - 1;
-  const int64_t blind = c >= 0 ? 0 : min(quotient(-c, tokens), regular);   // units that see nothing, one each
-  const int64_t n = regular - blind, b = c + tokens * (blind + 1) + kKeys - 1;
-  int64_t sum = blind;
+  const int tokens = a.tokens, c = s.m - s.n;
+  const int regular = units < all ? units : all - 1;
+  const int blind = c >= 0 ? 0 : min(-c / tokens, regular);   // units that see nothing
+  const int n = regular - blind, b = c + tokens * (blind + 1) + kKeys - 1;
+  int sum = units * a.unit_cost;
   if (a.token_shift < 0) {
-    sum += floor_sum(n, kKeys, tokens, b);
+    sum += static_cast<int>(floor_sum(n, kKeys, tokens, b));
   } else if (tokens >= kKeys) {
-    sum += n * (n - 1) / 2 * (tokens / kKeys) + n * (b / kKeys);
+    sum += static_cast<int>(static_cast<int64_t>(n) * (n - 1) / 2) * (tokens / kKeys) + n * (b / kKeys);
   } else {
-    // floor((tokens i + b) / kKeys) = floor((i + first) / r) with r = kKeys / tokens, first = floor(b / tokens);
-    // below x the quotients y / r add up to r q (q - 1) / 2 + q (x mod r), q = x / r.
+    // tokens divides the block: floor((tokens i + b) / kKeys) = floor((i + first) / r) with
+    // r = kKeys / tokens, first = floor(b / tokens); below x the quotients y / r add up to
+    // r q (q - 1) / 2 + q (x mod r), q = x / r.
     constexpr int kLog = kKeys == 128 ? 7 : 6;
     static_assert(1 << kLog == kKeys, "key blocks of 64 or 128");
-    const int64_t r = kKeys >> a.token_shift, first = b >> a.token_shift;
-    const auto below = [&](int64_t x) {
-      const int64_t q = x >> (kLog - a.token_shift);
-      return r * (q * (q - 1) / 2) + q * (x - q * r);
+    const int shift = kLog - a.token_shift, first = b >> a.token_shift;
+    const auto below = [&](int x) {
+      const int q = x >> shift;
+      return static_cast<int64_t>(q) * (q - 1) / 2 * (1 << shift) + static_cast<int64_t>(q) * (x - (q << shift));
     };
-    sum += below(first + n) - below(first);
+    sum += static_cast<int>(below(first + n) - below(first));
   }
-  if (units == all) sum += unit_weight<kKeys>(a, s, all - 1);
+  if (units == all) sum += unit_blocks<kKeys>(a, s, all - 1);
   return sum;
-}
-
-template <int kKeys>
-__device__ __forceinline__ int64_t head_weight(const AttentionArgs& a, const Sequence& s) {
-  return weight_before<kKeys>(a, s, unit_count(a, s));
 }
 
 // ------------------------------------------------------------------------- finding a CTA's work
 
+// Ranges of the line: the first total % ctas are one longer than the rest.
+struct Ranges {
+  int quotient, longer;
+  __device__ __forceinline__ Ranges(int total, int ctas) : quotient(total / ctas), longer(total - total / ctas * ctas) {}
+  __device__ __forceinline__ int begin(int c) const { return c * quotient + min(c, longer); }
+  __device__ __forceinline__ int holder(int position) const {
+    const int boundary = longer * (quotient + 1);
+    return position < boundary ? position / (quotient + 1) : longer + (position - boundary) / quotient;
+  }
+};
+
 struct WorkStart {
   int sequence;               // -1: nothing to do
-  int head, unit, block;
-  int64_t per, length;        // blocks per range, and of this one
-  int64_t position, before;   // of the range; of the first block of `unit`
+  Sequence seq;
+  int units;                  // of a head of the sequence
+  int head, unit, offset;     // offset: into the unit
+  int total, begin, length;   // of the line; the range
 };
 
 struct WorkScratch {
-  int64_t sums[32];
+  int sums[32];
   WorkStart start;
 };
 
-// Where range `range` starts: prefix sums over the sequences by all kThreads threads of the CTA.
+// Where this CTA's range starts: prefix sums over the sequences by all kThreads threads.
 template <int kKeys, int kThreads>
-__device__ __forceinline__ WorkStart find_range(const AttentionArgs& a, WorkScratch* scratch, int range) {
+__device__ __forceinline__ WorkStart find_range(const AttentionArgs& a, WorkScratch* scratch) {
   const int count = sequence_count(a);
   const int chunk = (count + kThreads - 1) / kThreads;
   const int lo = min(static_cast<int>(threadIdx.x) * chunk, count), hi = min(lo + chunk, count);
-  const auto weight = [&](int s) { return a.kv_heads * head_weight<kKeys>(a, sequence_of(a, s)); };
-  int64_t mine = 0;
-  for (int s = lo; s < hi; ++s) mine += weight(s);
-  int64_t upto = mine;   // inclusive over the warp
+  Sequence seq{};
+  int mine = 0, size = 0;
+  for (int s = lo; s < hi; ++s) {
+    seq = sequence_of(a, s);
+    const int units = unit_count(a, seq);
+    size = a.kv_heads * length_before<kKeys>(a, seq, units, units);
+    mine += size;
+  }
+  int upto = mine;   // inclusive over the warp
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t other = __shfl_up_sync(0xffffffffu, upto, o);
+    const int other = __shfl_up_sync(0xffffffffu, upto, o);
     if ((threadIdx.x & 31) >= o) upto += other;
   }
   if ((threadIdx.x & 31) == 31) scratch->sums[threadIdx.x >> 5] = upto;
+  WorkStart& start = scratch->start;
+  if (threadIdx.x == 0) start.sequence = -1;
   __syncthreads();
-  int64_t before = upto - mine, total = 0;
+  int before = upto - mine, total = 0;
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < static_cast<int>(threadIdx.x >> 5)) before += scratch->sums[w];
     total += scratch->sums[w];
   }
-  const int64_t per = quotient(total + a.ctas - 1, a.ctas);
-  const int64_t position = range * per;
-  WorkStart& start = scratch->start;
-  if (threadIdx.x == 0) start = WorkStart{-1, 0, 0, 0, per, 0, position, 0};
-  __syncthreads();
-  if (position >= before && position < before + mine) {
+  const Ranges ranges(total, a.ctas);
+  const int begin = ranges.begin(blockIdx.x), length = ranges.begin(blockIdx.x + 1) - begin;
+  if (length > 0 && begin >= before && begin < before + mine) {
     int s = lo;
-    int64_t size = mine;
-    for (; s < hi; ++s) {
-      size = hi - lo == 1 ? mine : weight(s);
-      if (position < before + size) break;
-      before += size;
+    if (hi - lo > 1) {
+      for (; s < hi; ++s) {
+        seq = sequence_of(a, s);
+        const int units = unit_count(a, seq);
+        size = a.kv_heads * length_before<kKeys>(a, seq, units, units);
+        if (begin < before + size) break;
+        before += size;
+      }
     }
-    const int64_t per_head = quotient(size, a.kv_heads);
-    start.sequence = s;
-    start.head = static_cast<int>(quotient(position - before, per_head));
-    start.length = min(per, total - position);
-    start.before = before + start.head * per_head;   // of the head, until the unit is known
+    const int per_head = size / a.kv_heads, head = (begin - before) / per_head;
+    start = WorkStart{s, seq, unit_count(a, seq), head, 0, begin - before - head * per_head, total, begin, length};
   }
   __syncthreads();
-  const WorkStart found = start;
+  WorkStart found = start;
   if (found.sequence < 0) return found;
   // The last unit that does not start behind the position, by all threads at once.
-  const Sequence seq = sequence_of(a, found.sequence);
-  const int64_t rest = position - found.before;
-  int low = 0, high = unit_count(a, seq);
+  int low = 0, high = found.units;
   while (true) {
     const int step = (high - low + kThreads - 1) / kThreads;
     const int mid = low + step * static_cast<int>(threadIdx.x), end = min(mid + step, high);
     __syncthreads();
     if (mid < high) {
-      const int64_t first = weight_before<kKeys>(a, seq, mid);
-      if (first <= rest && (end == high || rest < weight_before<kKeys>(a, seq, end)))
-        start.unit = mid, start.block = static_cast<int>(rest - first), start.before = found.before + first;
+      const int first = length_before<kKeys>(a, found.seq, mid, found.units);
+      if (first <= found.offset && (end == high || found.offset < length_before<kKeys>(a, found.seq, end, found.units)))
+        start.unit = mid, start.offset = found.offset - first;
     }
     __syncthreads();
     low = start.unit, high = min(low + step, high);
@@ -268,65 +280,104 @@ struct Segment {
   int head, unit;
   int block_begin, block_end;   // of the unit's blocks; none for rows that see no key
   bool opens, whole;            // starts at the unit's first block; is all of it
+  int first_cta, last_cta;      // of an opened unit
 };
 
-// Walks the segments of a CTA's range. Every role of a CTA walks for itself and sees the same ones.
+// Walks the segments of a CTA's range.
 template <int kKeys>
 struct SegmentWalk {
   const AttentionArgs& a;
-  int64_t left;      // blocks still to be handed out
+  Ranges ranges;
+  int position, end;   // on the line
   int sequence, units;
   Sequence seq;
-  int head, unit, block;
+  int head, unit, offset;
 
-  __device__ __forceinline__ SegmentWalk(const AttentionArgs& args, const WorkStart& start) : a(args), left(0), sequence(start.sequence) {
-    if (sequence < 0) return;
-    seq = sequence_of(a, sequence);
-    units = unit_count(a, seq);
-    left = start.length, head = start.head, unit = start.unit, block = start.block;
+  __device__ __forceinline__ SegmentWalk(const AttentionArgs& args, const WorkStart& start) : a(args), ranges(start.total, args.ctas) {
+    position = start.begin, end = start.sequence < 0 ? start.begin : start.begin + start.length;
+    sequence = start.sequence, seq = start.seq, units = start.units, head = start.head, unit = start.unit, offset = start.offset;
   }
 
   __device__ __forceinline__ bool next(Segment* out) {
-    if (left <= 0) return false;
-    int blocks = unit_blocks<kKeys>(a, seq, unit), weight = a.kind == kPrompt ? max(blocks, 1) : blocks;
-    while (block >= weight) {   // on to the next unit that counts; there is one while `left` > 0
-      block = 0;
-      if (++unit >= units) {
-        unit = 0;
-        if (++head >= a.kv_heads) {
-          head = 0;
-          do {
-            seq = sequence_of(a, ++sequence);
-            units = unit_count(a, seq);
-          } while (units == 0);
+    while (position < end) {
+      const int blocks = unit_blocks<kKeys>(a, seq, unit), length = unit_length(a, blocks);
+      const int from = offset, to = min(length, offset + end - position);
+      const int unit_position = position - from;
+      Segment g{seq, head, unit, max(from - a.unit_cost, 0), max(to - a.unit_cost, 0), false, false, 0, 0};
+      position += to - from;
+      offset = to;
+      if (to == length) {   // on to the next unit
+        offset = 0;
+        if (++unit >= units) {
+          unit = 0;
+          if (++head >= a.kv_heads && position < end) {
+            head = 0;
+            do {
+              seq = sequence_of(a, ++sequence);
+              units = unit_count(a, seq);
+            } while (units == 0);
+          }
         }
       }
-      blocks = unit_blocks<kKeys>(a, seq, unit), weight = a.kind == kPrompt ? max(blocks, 1) : blocks;
+      // A range may end within what a unit costs beside its blocks, or hold only such a piece of it.
+      if (blocks > 0 ? g.block_end > g.block_begin : length > 0 && to == length) {
+        g.opens = g.block_begin == 0, g.whole = g.opens && g.block_end == blocks;
+        g.first_cta = blockIdx.x, g.last_cta = g.whole ? blockIdx.x : ranges.holder(unit_position + length - 1);
+        *out = g;
+        return true;
+      }
     }
-    const int take = static_cast<int>(min(static_cast<int64_t>(weight - block), left));
-    *out = Segment{seq, head, unit, block, min(block + take, blocks), block == 0, take == weight};
-    block += take;
-    left -= take;
-    return true;
+    return false;
   }
 };
 
-// Where rows go: row `row` of a unit is the output row `out` (token * heads + head).
-__device__ __forceinline__ int64_t continued_row(const AttentionArgs& a, int cta, int row) {
-  return static_cast<int64_t>(cta) * a.unit_rows + row;
+// ------------------------------------------------------------------------------- partial results
+
+// Rows in front of slots; see AttentionArgs. prefix_units: of one head.
+__device__ __forceinline__ int64_t continued_slot(const AttentionArgs& a, int cta) { return static_cast<int64_t>(cta) * a.unit_rows; }
+__device__ __forceinline__ int prefix_units(const AttentionArgs& a) { return (a.q_rows * a.group + a.unit_rows - 1) / a.unit_rows; }
+__device__ __forceinline__ int64_t prefix_slot(const AttentionArgs& a, int unit, int head) {
+  return (a.ctas + static_cast<int64_t>(unit) * a.kv_heads + head) * a.unit_rows;
 }
-__device__ __forceinline__ int64_t opened_row(const AttentionArgs& a, const Sequence& s, int64_t out, int cta, int row) {
-  const int64_t first = static_cast<int64_t>(a.ctas) * a.unit_rows;
-  return first + (a.kind == kPrompt ? continued_row(a, cta, row) : s.source * static_cast<int64_t>(a.q_rows) * a.heads + out);
+__device__ __forceinline__ int64_t own_slot(const AttentionArgs& a, int request, int head, int unit) {
+  return (a.ctas + static_cast<int64_t>(prefix_units(a)) * a.kv_heads) * a.unit_rows +
+         (static_cast<int64_t>(request) * a.kv_heads + head) * a.group + unit * a.unit_rows;
 }
+__device__ __forceinline__ int own_pitch(const AttentionArgs& a, int unit) { return min(a.unit_rows, a.group - unit * a.unit_rows); }
+__device__ __forceinline__ int64_t prefix_record(const AttentionArgs& a, int unit, int head) { return static_cast<int64_t>(unit) * a.kv_heads + head; }
+__device__ __forceinline__ int64_t own_record(const AttentionArgs& a, int request, int head, int unit) {
+  const int units = (a.group + a.unit_rows - 1) / a.unit_rows;
+  return (static_cast<int64_t>(prefix_units(a)) + static_cast<int64_t>(request) * units + unit) * a.kv_heads + head;
+}
+
 __device__ __forceinline__ bool is_partial(const AttentionArgs& a, const Segment& g) { return a.kind == kShared || !g.whole; }
-__device__ __forceinline__ int64_t partial_row(const AttentionArgs& a, const Segment& g, int64_t out, int row) {
-  return g.opens ? opened_row(a, g.seq, out, blockIdx.x, row) : continued_row(a, blockIdx.x, row);
+
+// Slot of a segment's partial result, and the rows of the slot.
+__device__ __forceinline__ int64_t slot_of(const AttentionArgs& a, const Segment& g, int* pitch) {
+  *pitch = a.unit_rows;
+  if (!g.opens) return continued_slot(a, blockIdx.x);
+  if (a.kind == kPrompt) return continued_slot(a, a.ctas + blockIdx.x);
+  if (g.seq.source == 0) return prefix_slot(a, g.unit, g.head);
+  *pitch = own_pitch(a, g.unit);
+  return own_slot(a, g.seq.batch, g.head, g.unit);
 }
+
+// The record of an opened unit. To be called by one thread of the CTA for each segment, and, in a
+// prompt call, once before the first (`start`).
+__device__ __forceinline__ void start_records(const AttentionArgs& a) {
+  if (a.kind == kPrompt && a.cuts != nullptr) a.cuts[blockIdx.x] = CutRecord{};
+}
+__device__ __forceinline__ void record(const AttentionArgs& a, const Segment& g) {
+  if (!g.opens || !is_partial(a, g)) return;
+  const CutRecord r{g.first_cta, g.last_cta, min(a.unit_rows, g.seq.n * a.group - g.unit * a.unit_rows), g.seq.q_row, g.head, g.unit * a.unit_rows};
+  if (a.kind == kPrompt) a.cuts[blockIdx.x] = r;
+  else a.cuts[g.seq.source == 0 ? prefix_record(a, g.unit, g.head) : own_record(a, g.seq.batch, g.head, g.unit)] = r;
+}
+
 // Output row of row `flat` of a sequence's rows of a key head.
-__device__ __forceinline__ int64_t output_row(const AttentionArgs& a, const Sequence& s, int head, int flat) {
+__device__ __forceinline__ int64_t output_row(const AttentionArgs& a, int q_row, int head, int flat) {
   const int token = flat / a.group;
-  return static_cast<int64_t>(s.q_row + token) * a.heads + head * a.group + (flat - token * a.group);
+  return static_cast<int64_t>(q_row + token) * a.heads + head * a.group + (flat - token * a.group);
 }
 
 // The kernels: rows of a unit and CTAs that the machine holds at once, and launch. The key block of

@@ -52,9 +52,13 @@ __global__ void __launch_bounds__(kRows * 4) attention_simt_kernel(const Attenti
   grid_launch_dependents();
   grid_dependency_wait();
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  SegmentWalk<kKeys> walk(a, find_range<kKeys, kThreads>(a, &scratch, blockIdx.x));
+  SegmentWalk<kKeys> walk(a, find_range<kKeys, kThreads>(a, &scratch));
   Segment g;
+  if (threadIdx.x == 0) start_records(a);
   while (walk.next(&g)) {
+    if (threadIdx.x == 0) record(a, g);
+    int pitch_rows;
+    const int64_t slot = slot_of(a, g, &pitch_rows);
     const int row0 = g.unit * a.unit_rows;
     const int rows = min(a.unit_rows, g.seq.n * a.group - row0);
     __syncthreads();   // the last segment's readers are done
@@ -146,16 +150,14 @@ __global__ void __launch_bounds__(kRows * 4) attention_simt_kernel(const Attenti
     for (int i = 0; i < 4; ++i) {
       const int r = ty * 4 + i;
       if (r >= rows) continue;
-      const int64_t out = output_row(a, g.seq, g.head, row0 + r);
       if (is_partial(a, g)) {
-        const int64_t row = partial_row(a, g, out, r);
-        if (tx == 0) a.partial_ml[row] = make_float2(m[i], l[i]);
+        if (tx == 0) a.partial_ml[slot + r] = make_float2(m[i], l[i]);
 #pragma unroll
         for (int c = 0; c < 2; ++c)
-          if (tx * 4 + 64 * c < a.dim) store4(a.partial_o + row * a.dim + tx * 4 + 64 * c, o[i][c]);
+          if (tx * 4 + 64 * c < a.dim) store4(a.partial_o + slot * a.dim + (static_cast<int64_t>(tx + 16 * c) * pitch_rows + r) * 4, o[i][c]);
       } else {
         const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
-        float* y = static_cast<float*>(a.out) + out * a.dim;
+        float* y = static_cast<float*>(a.out) + output_row(a, g.seq.q_row, g.head, row0 + r) * a.dim;
 #pragma unroll
         for (int c = 0; c < 2; ++c)
           if (tx * 4 + 64 * c < a.dim)
@@ -193,6 +195,7 @@ void plan_attention_simt(AttentionArgs* a, int sms) {
   const int tile = rows_per_sequence <= 16 ? 16 : 64;
   a->tokens = tile / a->group;
   a->unit_rows = a->tokens > 0 ? a->tokens * a->group : tile;
+  a->unit_cost = 1;
   a->ctas = sms * (tile == 16 ? 3 : 2);
 }
 

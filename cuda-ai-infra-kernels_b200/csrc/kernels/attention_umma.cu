@@ -42,7 +42,8 @@ constexpr float kLazy = 8.f;        // growth of a maximum, in powers of two, th
 constexpr uint32_t kColS = 0, kColO = 256, kColStream = 128;   // TMEM columns
 
 struct UmmaAttentionArgs {
-  CUtensorMap q, k[2], v[2];
+  CUtensorMap q, k[2], v[2], out;
+  int boxed;   // a warp's 32 rows of the output are a box of `out`
   AttentionArgs a;
 };
 
@@ -65,8 +66,8 @@ struct SegmentEntry {
   int keys, ahead;         // from the first block on: keys of the sequence; keys that token t of the unit sees
                            // are ahead + t, cut to 0 .. keys
   int live_keys;           // of the last block
-  int partial;
-  int64_t partial_row;     // of the unit's first row, where rows follow one another; -1: by output row
+  int partial, pitch;
+  int64_t slot;            // of the partial result
 };
 constexpr int kEntries = 4;
 
@@ -83,8 +84,6 @@ struct Shared {   // behind the tiles
   WorkScratch scratch;
 };
 constexpr int kEntryReaders = 1 + 2 + 8;
-
-__device__ __forceinline__ int items_of(const SegmentEntry& e, int s) { return e.pair != 0 ? e.blocks : (e.blocks + 1 - s) / 2; }
 
 // A role's place in the ring of segments. Called by whole warps or by single threads.
 struct EntryReader {
@@ -139,15 +138,16 @@ __device__ __forceinline__ void segment_role(const UmmaAttentionArgs& p, const W
   SegmentWalk<kUmmaKeyBlock> walk(a, start);
   Segment g;
   bool ok = true;
+  if (lane == 0) start_records(a);
   // Blocks whose last rows have to be cleared, at most kDelay segments behind the newest: the slot of
   // the ring and the live rows.
   constexpr uint32_t kDelay = 2;
-  int slot_of[kDelay] = {-1, -1}, live_of[kDelay] = {0, 0};
+  int dirty[kDelay] = {-1, -1}, live_of[kDelay] = {0, 0};
   uint32_t loads = 0, raw_phase = 0;
   const auto clear = [&](int i) {
-    const int slot = slot_of[i];
+    const int slot = dirty[i];
     if (slot < 0) return;
-    slot_of[i] = -1;
+    dirty[i] = -1;
     ok = __all_sync(0xffffffffu, ok && mbar_wait(&b->raw[slot], raw_phase >> slot & 1, kSiteAttention));
     raw_phase ^= 1u << slot;
     if (!ok) return;
@@ -174,7 +174,8 @@ __device__ __forceinline__ void segment_role(const UmmaAttentionArgs& p, const W
       e.ahead = a.kind == kShared || a.causal == 0 ? e.keys : g.seq.m - g.seq.n + token0 + 1 - first;
       e.live_keys = min(kTile, g.seq.m - (g.block_end - 1) * kTile);
       e.partial = is_partial(a, g);
-      e.partial_row = g.opens && a.kind == kShared ? -1 : partial_row(a, g, 0, 0);
+      e.slot = slot_of(a, g, &e.pitch);
+      if (lane == 0) record(a, g);
     } else {
       e.blocks = -1;
     }
@@ -189,7 +190,7 @@ __device__ __forceinline__ void segment_role(const UmmaAttentionArgs& p, const W
     }
     if (e.blocks > 0) {
       loads += 2 * e.blocks;
-      if (e.live_keys < kTile) slot_of[count % kDelay] = (loads - 1) % S::kSlots, live_of[count % kDelay] = e.live_keys;
+      if (e.live_keys < kTile) dirty[count % kDelay] = (loads - 1) % S::kSlots, live_of[count % kDelay] = e.live_keys;
     }
   }
 }
@@ -374,42 +375,17 @@ __device__ __forceinline__ void softmax_block(uint32_t s_at, uint32_t o_at, int 
   tmem_st_wait();
 }
 
-// Finished columns [column, column + 32) of a warp's 32 rows. Each thread holds its row's, and rows lie
-// far apart: stored from the registers, every instruction would touch 32 lines of memory, which the
-// load/store unit takes one per cycle (8600 cycles a unit). So they are turned through the warp's 4 KiB
-// of shared memory, in 16-byte pieces whose place is permuted by the row to keep the banks apart;
-// then 4 or 8 lanes store each row's piece of 64 (16-bit) or 128 bytes. at: element offset of the
-// lane's row, -1: not there.
+// A warp's 32 finished rows, 64 columns at a time. Each thread holds its own row, and rows lie far apart:
+// stored from the registers, every instruction would touch 32 lines of memory, which the load/store
+// unit takes one per cycle. Where the 32 rows are all there they are laid out in the warp's 4 KiB of
+// shared memory, in the 128-byte swizzle, and leave as one box.
 template <bool kBf16>
-__device__ __forceinline__ void store_columns(const AttentionArgs& a, bool partial, uint4* stage, int lane, int64_t at, int column,
-                                              const float (&y)[32]) {
-  const int pieces = partial ? 8 : 4;
-  if (partial) {
+__device__ __forceinline__ void stage_columns(uint8_t* stage, int lane, int half, const float (&y)[32]) {
+  uint4* row = reinterpret_cast<uint4*>(stage + lane * 128);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      stage[lane * 8 + (i ^ (lane & 7))] = make_uint4(__float_as_uint(y[4 * i]), __float_as_uint(y[4 * i + 1]), __float_as_uint(y[4 * i + 2]),
-                                                      __float_as_uint(y[4 * i + 3]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      stage[lane * 8 + (i ^ (lane & 7))] = make_uint4(pack<kBf16>(y[8 * i], y[8 * i + 1]), pack<kBf16>(y[8 * i + 2], y[8 * i + 3]),
-                                                      pack<kBf16>(y[8 * i + 4], y[8 * i + 5]), pack<kBf16>(y[8 * i + 6], y[8 * i + 7]));
-  }
-  __syncwarp();
-  const int piece = lane & (pieces - 1), width = partial ? 4 : 8;   // elements of a piece
-  const bool inside = column + piece * width < a.dim;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int row = (partial ? j * 4 : j * 8) + lane / pieces;
-    if (!partial && j >= 4) break;
-    const int64_t to = __shfl_sync(0xffffffffu, at, row);
-    const uint4 v = stage[row * 8 + (piece ^ (row & 7))];
-    if (to >= 0 && inside) {
-      if (partial) *reinterpret_cast<uint4*>(a.partial_o + to + column + piece * 4) = v;
-      else *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + to + column + piece * 8) = v;
-    }
-  }
-  __syncwarp();
+  for (int i = 0; i < 4; ++i)
+    row[(half * 4 + i) ^ (lane & 7)] = make_uint4(pack<kBf16>(y[8 * i], y[8 * i + 1]), pack<kBf16>(y[8 * i + 2], y[8 * i + 3]),
+                                                  pack<kBf16>(y[8 * i + 4], y[8 * i + 5]), pack<kBf16>(y[8 * i + 6], y[8 * i + 7]));
 }
 
 template <bool kBf16>
@@ -421,7 +397,7 @@ __device__ __forceinline__ void softmax_role(const UmmaAttentionArgs& p, Shared*
   const uint32_t lanes = static_cast<uint32_t>(warp_row) << 16;
   const uint32_t s_at = tmem + lanes + kColS + s * kColStream, o_at = tmem + lanes + kColO + s * kColStream;
   const uint32_t other_o_at = tmem + lanes + kColO + (s ^ 1) * kColStream;
-  uint4* stage = reinterpret_cast<uint4*>(staging + (threadIdx.x >> 5) * 4096);
+  uint8_t* stage = staging + (threadIdx.x >> 5) * 4096;
   const int tile_rows = a.unit_rows / 2, tile_tokens = a.tokens / 2;
   const int token_r = r / a.group, head_r = r - token_r * a.group, token_warp = warp_row / a.group;   // within the tile
   const int chunks = (a.dim + 31) / 32;
@@ -442,16 +418,16 @@ __device__ __forceinline__ void softmax_role(const UmmaAttentionArgs& p, Shared*
     const bool pair = entry->pair != 0, partial = entry->partial != 0;
     const int keys = entry->keys, ahead = entry->ahead, tokens = entry->tokens;
     const int token0 = pair && s == 1 ? tile_tokens : 0;   // of the tile within the unit
-    const int64_t out_row = static_cast<int64_t>(entry->q_row + token0 + token_r) * a.heads + entry->head * a.group + head_r;
-    int64_t at = out_row;
-    if (partial) {
-      at = entry->partial_row >= 0 ? entry->partial_row + (pair && s == 1 ? tile_rows : 0) + r
-                                   : static_cast<int64_t>(a.ctas) * a.unit_rows + entry->source * static_cast<int64_t>(a.q_rows) * a.heads + out_row;
-    }
+    const int q_row = entry->q_row + token0, head = entry->head * a.group;
+    const int64_t slot = entry->slot;
+    const int pitch = entry->pitch, slot_row = (pair && s == 1 ? tile_rows : 0) + r;
     __syncwarp();
     if (lane == 0) reader.release();
     else ++reader.count;
-    if (blocks < 0) return;
+    if (blocks < 0) {
+      if (lane == 0) tma_store_wait_read<0>();   // shared memory must outlive the copies' reads
+      return;
+    }
     const bool live = r < tile_rows && token0 + token_r < tokens;
     const bool warp_live = warp_row < tile_rows && token0 + token_warp < tokens;   // some row of the warp is there
     const int items = pair ? blocks : (blocks + 1 - s) / 2;
@@ -495,28 +471,64 @@ __device__ __forceinline__ void softmax_role(const UmmaAttentionArgs& p, Shared*
     }
     tcgen05_fence_after_sync();
     if (ok && warp_live && (pair || s == 0 || joined)) {
-      if (partial && live && (pair || s == 0)) a.partial_ml[at] = make_float2(base, total);
+      if (partial && live && (pair || s == 0)) a.partial_ml[slot + slot_row] = make_float2(base, total);
       const float inv = partial ? 1.f : (total == 0.f ? 0.f : 1.f / total);
-      const float f0 = mine * inv, f1 = other * inv;
-      const int64_t element = live ? at * a.dim : -1;
-      for (int c = joined ? s : 0; c < chunks; c += joined ? 2 : 1) {
+      const uint64_t f0 = pack_f32x2(mine * inv, mine * inv), f1 = pack_f32x2(other * inv, other * inv);
+      const bool boxed = !partial && p.boxed != 0 && warp_row + 32 <= tile_rows && token0 + (warp_row + 31) / a.group < tokens;
+      float* o_slot = a.partial_o + slot * a.dim + slot_row * 4;
+      uint16_t* o_row = static_cast<uint16_t*>(a.out) + (static_cast<int64_t>(q_row + token_r) * a.heads + head + head_r) * a.dim;
+      // Two warps that own the same rows take 64 columns each.
+      for (int c = joined ? 2 * s : 0; c < (joined ? min(chunks, 2 * s + 2) : chunks); ++c) {
         float y[32];
         if (blocks > 0) {
           load_columns(o_at + 32 * c, y);
-          // A row that saw nothing keeps its zeros whatever its accumulator holds.
-#pragma unroll
-          for (int i = 0; i < 32; ++i) y[i] = total == 0.f ? 0.f : y[i] * f0;
           if (joined) {
             float z[32];
             load_columns(other_o_at + 32 * c, z);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) y[i] = total == 0.f ? 0.f : y[i] + z[i] * f1;
+            for (int i = 0; i < 32; i += 2) {
+              const uint64_t v = fma_f32x2(pack_f32x2(z[i], z[i + 1]), f1, 0);
+              const float2 w = unpack_f32x2(fma_f32x2(pack_f32x2(y[i], y[i + 1]), f0, v));
+              y[i] = w.x, y[i + 1] = w.y;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float2 w = unpack_f32x2(fma_f32x2(pack_f32x2(y[i], y[i + 1]), f0, 0));
+              y[i] = w.x, y[i + 1] = w.y;
+            }
           }
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) y[i] = 0.f;
         }
-        store_columns<kBf16>(a, partial, stage, lane, element, 32 * c, y);
+        if (boxed) {
+          if ((c & 1) == 0) {   // the box's last copy has been read
+            if (lane == 0) tma_store_wait_read<0>();
+            __syncwarp();
+          }
+          stage_columns<kBf16>(stage, lane, c & 1, y);
+          if ((c & 1) == 1 || c + 1 == chunks) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              const int token = warp_row / a.group;
+              tma_store_3d(&p.out, stage, (c & ~1) * 32, head + warp_row - token * a.group, q_row + token);
+              tma_store_commit();
+            }
+          }
+        } else if (live && partial) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (32 * c + 4 * i < a.dim)
+              *reinterpret_cast<float4*>(o_slot + static_cast<int64_t>(8 * c + i) * pitch * 4) = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+        } else if (live) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (32 * c + 8 * i < a.dim)
+              *reinterpret_cast<uint4*>(o_row + 32 * c + 8 * i) = make_uint4(pack<kBf16>(y[8 * i], y[8 * i + 1]), pack<kBf16>(y[8 * i + 2], y[8 * i + 3]),
+                                                                             pack<kBf16>(y[8 * i + 4], y[8 * i + 5]), pack<kBf16>(y[8 * i + 6], y[8 * i + 7]));
+        }
       }
     }
     tcgen05_fence_before_sync();
@@ -545,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_umma_kernel(const __gri
     mbar_init_fence();
   }
   if (threadIdx.x == 256) {
-    prefetch_tensormap(&p.q);
+    prefetch_tensormap(&p.q), prefetch_tensormap(&p.out);
     for (int i = 0; i < (p.a.kind == kShared ? 2 : 1); ++i) prefetch_tensormap(&p.k[i]), prefetch_tensormap(&p.v[i]);
   }
   if (warp == 9) {
@@ -558,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_umma_kernel(const __gri
   const uint32_t tmem = b.tmem;
   grid_launch_dependents();   // after the allocation: a following kernel may want tensor memory too
   grid_dependency_wait();
-  const WorkStart start = find_range<kUmmaKeyBlock, kThreads>(p.a, &b.scratch, blockIdx.x);
+  const WorkStart start = find_range<kUmmaKeyBlock, kThreads>(p.a, &b.scratch);
   if (warp < 8) {
     registers_raise<kSoftmaxRegisters>();
     softmax_role<kBf16>(p, &b, smem + S::kStaging, tmem);
@@ -610,6 +622,7 @@ void plan_attention_umma(AttentionArgs* a, int sms) {
   // Tiles hold whole tokens: a copy brings (dim, group, tokens) boxes.
   a->tokens = 2 * (kTile / a->group);
   a->unit_rows = a->tokens * a->group;
+  a->unit_cost = 1;
   a->ctas = sms;
 }
 
@@ -633,6 +646,12 @@ int launch_attention_umma(const AttentionArgs& a, cudaStream_t s) {
       p.k[i] = p.v[i] = p.q;
     }
   }
+  // A warp's rows are a box where they are whole tokens or lie within one.
+  p.boxed = (a.group <= 32 ? 32 % a.group : a.group % 32) == 0;
+  const uint64_t out_strides[2] = {static_cast<uint64_t>(a.dim) * 2, static_cast<uint64_t>(a.heads) * a.dim * 2};
+  const uint32_t out_box[3] = {64, static_cast<uint32_t>(a.group < 32 ? a.group : 32), static_cast<uint32_t>(a.group < 32 ? 32 / a.group : 1)};
+  if (p.boxed != 0) ok = ok && make_tensor_map_16bit(&p.out, a.out, 3, dims, out_strides, out_box, bf16);
+  else p.out = p.q;
   if (!ok) return B200_ERR_INVALID_PROBLEM;
   if (a.dim <= 64) return bf16 ? launch<64, true>(p, s) : launch<64, false>(p, s);
   return bf16 ? launch<128, true>(p, s) : launch<128, false>(p, s);
