@@ -1,18 +1,20 @@
 // Attention for 16-bit operands on the 5th-generation tensor cores.
 //
-// For a tile of 128 rows and a block of 128 keys: S = Q K^T into tensor memory (tcgen05.mma, both
-// operands in shared memory), the row maxima and P = 2^(scale S - m) in registers, one thread per
-// row, P back into tensor memory as a 16-bit operand in the columns that held S, and O += P V with P
-// read from there. O stays in tensor memory for the whole unit. P is rounded to the operand type
-// (relative 2^-9 or 2^-12 per probability, of the size of the output's own rounding); the denominator
-// adds up the unrounded FP32 values.
+// For a tile of 128 rows and 64 keys: S = Q K^T into tensor memory (tcgen05.mma, both operands in
+// shared memory), the row maxima and P = 2^(scale S - m) in registers, one thread per row, P back into
+// tensor memory as a 16-bit operand in columns that held S, and O += P V with P read from there. O
+// stays in tensor memory for the whole unit. P is rounded to the operand type (relative 2^-9 or 2^-12
+// per probability, of the size of the output's own rounding); the denominator adds up the unrounded
+// FP32 values.
 //
-// The products of one block take about as long as its exponentials, and each waits for the other.
-// Two streams therefore alternate, each with its own S and O: the tensor pipe works for one while
-// the warps work for the other. The streams are the two row tiles of a unit of 256 rows, over the
-// same blocks of keys; or, where a unit has at most one tile of rows (a decoding request, a short
-// prompt), the even and the odd blocks for the same tile, joined at the end: thread r of both groups
-// of warps owns row r and may read both accumulators.
+// Two streams, each with its own group of four warps, O and S: the two row tiles of a unit of 256
+// rows, over the same blocks of 128 keys; or, where a unit has at most one tile of rows (a decoding
+// request, a short prompt), the even and the odd blocks for the same tile, joined at the end: thread r
+// of both groups of warps owns row r and may read both accumulators. Each stream has two S: while the
+// warps work on one half block of 64 keys, the tensor pipe multiplies the P of the half before and
+// fills its place with the scores of the half after, so that neither waits for the other. (One S of
+// 128 keys per stream left the warps idle during the products: 4400 cycles per block of both streams
+// against the pipe's 2048.)
 //
 // The maximum is followed lazily: O and the denominator are rescaled only when a row's maximum has
 // grown by more than 2^8 since the last time, which the first block or two settle. Until then
@@ -39,7 +41,8 @@ static_assert(256 * kSoftmaxRegisters + 128 * kOtherRegisters <= kThreads * 168,
 constexpr int kTile = 128;          // rows of a tile, keys of a block
 constexpr float kMinusInf = -__builtin_huge_valf();
 constexpr float kLazy = 8.f;        // growth of a maximum, in powers of two, that forces a rescale
-constexpr uint32_t kColS = 0, kColO = 256, kColStream = 128;   // TMEM columns
+constexpr int kHalf = 64;           // keys of one S
+constexpr uint32_t kColS = 0, kColO = 256, kColStream = 128, kColHalf = 64;   // TMEM columns
 
 struct UmmaAttentionArgs {
   CUtensorMap q, k[2], v[2], out;
@@ -65,6 +68,7 @@ struct SegmentEntry {
   int k_row, batch, source, head;   // k_row: of the first block
   int keys, ahead;         // from the first block on: keys of the sequence; keys that token t of the unit sees
                            // are ahead + t, cut to 0 .. keys
+  int halves;              // half blocks that some row sees: 2 * blocks, or one less
   int live_keys;           // of the last block
   int partial, pitch;
   int64_t slot;            // of the partial result
@@ -75,7 +79,8 @@ struct Shared {   // behind the tiles
   uint64_t full[8], empty[8], raw[8];
   uint64_t entry_full[kEntries], entry_empty[kEntries];
   uint64_t q_full, q_empty;
-  uint64_t s_full[2], p_ready[2];
+  uint64_t s_full[2][2], p_ready[2][2];   // [stream][half]
+  uint64_t drained[2];         // all products but the last half's are in the accumulator
   uint64_t o_full[2], o_empty[2];
   uint64_t exchanged;          // eight warps have written, then eight have read
   uint32_t tmem;
@@ -84,6 +89,14 @@ struct Shared {   // behind the tiles
   WorkScratch scratch;
 };
 constexpr int kEntryReaders = 1 + 2 + 8;
+
+// Half blocks of a stream: all of the segment's, or those of every other block.
+__device__ __forceinline__ int items_of(const SegmentEntry& e, int s) {
+  if (e.pair != 0) return e.halves;
+  const int own_blocks = (e.blocks + 1 - s) / 2;
+  const bool owns_last = e.blocks > 0 && ((e.blocks - 1) & 1) == s;
+  return 2 * own_blocks - (owns_last ? 2 * e.blocks - e.halves : 0);
+}
 
 // A role's place in the ring of segments. Called by whole warps or by single threads.
 struct EntryReader {
@@ -172,6 +185,11 @@ __device__ __forceinline__ void segment_role(const UmmaAttentionArgs& p, const W
       e.batch = g.seq.batch, e.source = g.seq.source, e.head = g.head;
       e.keys = g.seq.m - first;
       e.ahead = a.kind == kShared || a.causal == 0 ? e.keys : g.seq.m - g.seq.n + token0 + 1 - first;
+      e.halves = 2 * e.blocks;
+      if (e.blocks > 0) {   // the unit's last row sees most
+        const int seen = clamp_int(e.ahead + min(a.tokens, e.tokens) - 1, 0, e.keys);
+        if (seen <= e.blocks * kTile - kHalf) --e.halves;
+      }
       e.live_keys = min(kTile, g.seq.m - (g.block_end - 1) * kTile);
       e.partial = is_partial(a, g);
       e.slot = slot_of(a, g, &e.pitch);
@@ -239,7 +257,7 @@ template <int kDim, bool kBf16>
 __device__ __forceinline__ void mma_role(const UmmaAttentionArgs& p, uint8_t* smem, Shared* b, uint32_t tmem, int s) {
   using S = Smem<kDim>;
   const AttentionArgs& a = p.a;
-  constexpr uint32_t kIdescS = umma_idesc_f16(kTile, kTile, kBf16, false, false);
+  constexpr uint32_t kIdescS = umma_idesc_f16(kTile, kHalf, kBf16, false, false);
   const uint32_t idesc_o = umma_idesc_f16(kTile, (a.dim + 15) / 16 * 16, kBf16, false, true);
   const int steps = (a.dim + 15) / 16;   // of 16 along the head dimension; what lies behind it reads as zero
   const uint64_t q_desc[2] = {umma_smem_desc(smem_u32(smem), 16, 1024, kUmmaSwizzle128B),
@@ -248,11 +266,12 @@ __device__ __forceinline__ void mma_role(const UmmaAttentionArgs& p, uint8_t* sm
   const uint64_t v_desc = umma_smem_desc(smem_u32(smem) + 2 * S::kTileBytes, S::kHalfBytes, 1024, kUmmaSwizzle128B);
   const uint32_t s_at = tmem + kColS + s * kColStream, o_at = tmem + kColO + s * kColStream;
   EntryReader reader{b};
-  uint32_t load = 0, segment = 0, item = 0, own_segment = 0;
+  uint32_t load = 0, segment = 0, own_segment = 0, p_phase = 0;   // p_phase: a bit per half
   while (true) {
     const SegmentEntry* entry = reader.wait();
     const int blocks = entry->blocks;
     const bool pair = entry->pair != 0;
+    const int items = items_of(*entry, s);
     reader.release();
     if (!reader.ok || blocks < 0) return;
     if (blocks == 0) continue;
@@ -265,41 +284,46 @@ __device__ __forceinline__ void mma_role(const UmmaAttentionArgs& p, uint8_t* sm
       if (!pair) mbar_arrive_relaxed(&b->empty[slot]);
       umma_commit(&b->empty[slot]);
     };
-    const auto scores = [&](int block) {
-      const uint32_t at = load + 2 * block, slot = at % S::kSlots;
-      if (!mbar_wait(&b->full[slot], at / S::kSlots & 1, kSiteAttention)) return false;
-      tcgen05_fence_after_sync();
-      const uint64_t qd = q_desc[pair ? s : 0], kd = umma_desc_advance(k_desc, slot * S::kTileBytes);
+    const auto arrived = [&](uint32_t at) { return mbar_wait(&b->full[at % S::kSlots], at / S::kSlots & 1, kSiteAttention); };
+    // Item j is half j & 1 of block first + (j >> 1) * step_blocks.
+    const auto load_of = [&](int j) { return load + 2 * (first + (j >> 1) * step_blocks); };
+    const auto scores = [&](int j) {   // K is there
+      const uint32_t slot = load_of(j) % S::kSlots, half = j & 1;
+      const uint64_t qd = q_desc[pair ? s : 0], kd = umma_desc_advance(k_desc, slot * S::kTileBytes + half * kHalf * 128);
 #pragma unroll
       for (int step = 0; step < kDim / 16; ++step) {
         if (step >= steps) break;
         const uint32_t offset = (step >> 2) * S::kHalfBytes + (step & 3) * 32;
-        umma_f16(s_at, umma_desc_advance(qd, offset), umma_desc_advance(kd, offset), kIdescS, step > 0);
+        umma_f16(s_at + half * kColHalf, umma_desc_advance(qd, offset), umma_desc_advance(kd, offset), kIdescS, step > 0);
       }
-      umma_commit(&b->s_full[s]);
-      release(slot);
-      if (block + step_blocks >= blocks) umma_commit(&b->q_empty);
-      return true;
+      umma_commit(&b->s_full[s][half]);
+      if (half == 1 || j + 1 == items) release(slot);
+      if (j + 1 == items) umma_commit(&b->q_empty);
     };
-    if (first >= blocks) {   // nothing for this stream
+    if (items == 0) {   // nothing for this stream
       mbar_arrive(&b->q_empty);
     } else {
-      if (!scores(first)) return;
-      for (int block = first; block < blocks; block += step_blocks) {
-        const uint32_t at = load + 2 * block + 1, slot = at % S::kSlots;
-        if (!mbar_wait(&b->full[slot], at / S::kSlots & 1, kSiteAttention)) return;
-        if (block == first && !mbar_wait(&b->o_empty[s], (own_segment & 1) ^ 1, kSiteAttention)) return;
-        if (!mbar_wait(&b->p_ready[s], item & 1, kSiteAttention)) return;
-        ++item;
+      if (!arrived(load_of(0))) return;
+      tcgen05_fence_after_sync();
+      scores(0);
+      if (items > 1) scores(1);
+      for (int j = 0; j < items; ++j) {
+        const uint32_t slot = (load_of(j) + 1) % S::kSlots, half = j & 1;
+        // A wait costs a few hundred cycles even when it is over already: everything but P is waited for
+        // before P, and what follows P is issued in one go.
+        if (half == 0 && (!arrived(load_of(j) + 1) || (j + 2 < items && !arrived(load_of(j + 2))))) return;
+        if (j == 0 && !mbar_wait(&b->o_empty[s], (own_segment & 1) ^ 1, kSiteAttention)) return;
+        if (!mbar_wait(&b->p_ready[s][half], p_phase >> half & 1, kSiteAttention)) return;
+        p_phase ^= 1u << half;
         tcgen05_fence_after_sync();
-        const uint64_t vd = umma_desc_advance(v_desc, slot * S::kTileBytes);
+        const uint64_t vd = umma_desc_advance(v_desc, slot * S::kTileBytes + half * kHalf * 128);
 #pragma unroll
-        for (int step = 0; step < kTile / 16; ++step)
-          umma_f16_tmem_a(o_at, s_at + step * 8, umma_desc_advance(vd, step * 2048), idesc_o, block != first || step > 0);
-        const bool last = block + step_blocks >= blocks;
-        if (last) umma_commit(&b->o_full[s]);
-        else if (!scores(block + step_blocks)) return;
-        release(slot);
+        for (int step = 0; step < kHalf / 16; ++step)
+          umma_f16_tmem_a(o_at, s_at + half * kColHalf + step * 8, umma_desc_advance(vd, step * 2048), idesc_o, j > 0 || step > 0);
+        if (j + 2 < items) scores(j + 2);
+        if (j + 2 == items) umma_commit(&b->drained[s]);
+        if (j + 1 == items) umma_commit(&b->o_full[s]);
+        if (half == 1 || j + 1 == items) release(slot);
       }
       ++own_segment;
     }
@@ -314,26 +338,26 @@ struct RowState {
   float m, l;   // base of the exponentials (scaled, base 2) and denominator
 };
 
-template <bool kBf16, bool kMasked>
-__device__ __forceinline__ void softmax_block(uint32_t s_at, uint32_t o_at, int chunks, int seen, float scale, bool first, RowState* row) {
-  float x[kTile];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_at + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&x[32 * c]));
+// One half block. `settled` waits until the products of the half before are in O.
+template <bool kBf16, bool kMasked, class Settled>
+__device__ __forceinline__ void softmax_half(uint32_t s_at, uint32_t o_at, int chunks, int seen, float scale, bool first, RowState* row,
+                                             const Settled& settled) {
+  float x[kHalf];
+  tmem_ld_32x32(s_at, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
+  tmem_ld_32x32(s_at + 32, *reinterpret_cast<uint32_t(*)[32]>(&x[32]));
   tmem_ld_wait();
   loaded(x);
+  float top[4] = {kMinusInf, kMinusInf, kMinusInf, kMinusInf};
   if (kMasked) {
 #pragma unroll
-    for (int i = 0; i < kTile; ++i)
+    for (int i = 0; i < kHalf; ++i)
       if (i >= seen) x[i] = kMinusInf;   // chosen, not added: the product may be NaN
   }
-  float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-  for (int i = 4; i < kTile - 4; i += 8) {
+  for (int i = 0; i < kHalf; i += 8) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) top[j] = max3(top[j], x[i + j], x[i + 4 + j]);
   }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], x[kTile - 4 + j]);
   const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
   if (first) {
     row->m = m;
@@ -344,6 +368,7 @@ __device__ __forceinline__ void softmax_block(uint32_t s_at, uint32_t o_at, int 
       const float keep = grown ? exp2_fast(row->m - next) : 1.f;
       row->l *= keep;
       row->m = next;
+      settled();
       for (int c = 0; c < 2 * chunks; ++c) {
         float o[16];
         tmem_ld_32x16(o_at + 16 * c, *reinterpret_cast<uint32_t(*)[16]>(&o));
@@ -359,7 +384,7 @@ __device__ __forceinline__ void softmax_block(uint32_t s_at, uint32_t o_at, int 
   const uint64_t scale2 = pack_f32x2(scale, scale), base2 = pack_f32x2(-base, -base);
   uint64_t sum[2] = {0, 0};
 #pragma unroll
-  for (int part = 0; part < 4; ++part) {
+  for (int part = 0; part < 2; ++part) {
     uint32_t packed[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -403,7 +428,7 @@ __device__ __forceinline__ void softmax_role(const UmmaAttentionArgs& p, Shared*
   const int chunks = (a.dim + 31) / 32;
   EntryReader reader{b};
   bool ok = true;
-  uint32_t item = 0, o_count[2] = {0, 0}, met = 0;
+  uint32_t s_phase = 0, drain_phase = 0, o_count[2] = {0, 0}, met = 0;
   // All eight warps; a bounded wait, which a plain barrier has not.
   const auto meet = [&]() {
     __syncwarp();
@@ -420,6 +445,7 @@ __device__ __forceinline__ void softmax_role(const UmmaAttentionArgs& p, Shared*
     const int token0 = pair && s == 1 ? tile_tokens : 0;   // of the tile within the unit
     const int q_row = entry->q_row + token0, head = entry->head * a.group;
     const int64_t slot = entry->slot;
+    const int items = ok ? items_of(*entry, s) : 0;
     const int pitch = entry->pitch, slot_row = (pair && s == 1 ? tile_rows : 0) + r;
     __syncwarp();
     if (lane == 0) reader.release();
@@ -430,24 +456,34 @@ __device__ __forceinline__ void softmax_role(const UmmaAttentionArgs& p, Shared*
     }
     const bool live = r < tile_rows && token0 + token_r < tokens;
     const bool warp_live = warp_row < tile_rows && token0 + token_warp < tokens;   // some row of the warp is there
-    const int items = pair ? blocks : (blocks + 1 - s) / 2;
     RowState row{kMinusInf, 0.f};
     const int seen = live ? clamp_int(ahead + token0 + token_r, 0, keys) : 0;
     // All rows of the warp that are there see at least what its first row sees.
     const int seen_by_all = clamp_int(ahead + token0 + token_warp, 0, keys);
-    for (int i = 0; i < items; ++i) {
-      const int key0 = (pair ? i : 2 * i + s) * kTile;
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(&b->s_full[s], item & 1, kSiteAttention));
-      ++item;
+    for (int j = 0; j < items; ++j) {
+      const uint32_t half = j & 1;
+      const int key0 = (pair ? j : 4 * (j >> 1) + 2 * s + (j & 1)) * kHalf;
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(&b->s_full[s][half], s_phase >> half & 1, kSiteAttention));
+      s_phase ^= 1u << half;
       if (ok && warp_live) {
         tcgen05_fence_after_sync();
-        if (key0 + kTile <= seen_by_all) softmax_block<kBf16, false>(s_at, o_at, chunks, 0, a.scale_log2, i == 0, &row);
-        else softmax_block<kBf16, true>(s_at, o_at, chunks, seen - key0, a.scale_log2, i == 0, &row);
+        // Scores of the half after are issued behind the products of the half before; the last half
+        // has a signal of its own.
+        const auto settled = [&]() {
+          const bool more = j + 1 < items;
+          ok = __all_sync(0xffffffffu, ok && mbar_wait(more ? &b->s_full[s][half ^ 1] : &b->drained[s],
+                                                       more ? s_phase >> (half ^ 1) & 1 : drain_phase, kSiteAttention));
+          tcgen05_fence_after_sync();
+        };
+        const uint32_t at = s_at + half * kColHalf;
+        if (key0 + kHalf <= seen_by_all) softmax_half<kBf16, false>(at, o_at, chunks, 0, a.scale_log2, j == 0, &row, settled);
+        else softmax_half<kBf16, true>(at, o_at, chunks, seen - key0, a.scale_log2, j == 0, &row, settled);
         tcgen05_fence_before_sync();
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&b->p_ready[s]);
+      if (lane == 0) mbar_arrive(&b->p_ready[s][half]);
     }
+    if (items > 1) drain_phase ^= 1;
     // Rows of one tile that two streams worked on: the same thread of both warp groups owns them, and
     // each finishes every other 32 columns.
     const bool joined = !pair && blocks > 1;
@@ -551,7 +587,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_umma_kernel(const __gri
     for (int i = 0; i < kEntries; ++i) mbar_init(&b.entry_full[i], 1), mbar_init(&b.entry_empty[i], kEntryReaders);
     mbar_init(&b.q_full, 1), mbar_init(&b.q_empty, 2), mbar_init(&b.exchanged, 8);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&b.s_full[s], 1), mbar_init(&b.p_ready[s], 4);
+      for (int h = 0; h < 2; ++h) mbar_init(&b.s_full[s][h], 1), mbar_init(&b.p_ready[s][h], 4);
+      mbar_init(&b.drained[s], 1);
       mbar_init(&b.o_full[s], 1), mbar_init(&b.o_empty[s], 8);
     }
     mbar_init_fence();
