@@ -9,9 +9,9 @@
 // is: a decoding batch fills a tile with requests and heads as a prompt fills it with tokens.
 //
 // A unit is `unit_rows` such rows of one key head; its keys are cut in blocks, 128 or 64 keys each. All
-// units, in the order sequence, head, unit, are laid end to end, each as long as its blocks plus
-// `unit_cost` for what a unit costs beside them, and the line is dealt out in equal contiguous
-// ranges, one per CTA, whatever the lengths are. (One CTA per unit, longest first, left the tensor
+// units, in the order sequence, head, unit, are laid end to end, each as long as its blocks (twice,
+// where the kernel works on two tiles of rows) plus `unit_cost` for what a unit costs beside them, and
+// the line is dealt out in equal contiguous ranges, one per CTA, whatever the lengths are. (One CTA per unit, longest first, left the tensor
 // pipe idle at the start and end of every unit and the machine uneven at the end of a call.) A unit
 // that lies inside one range is finished by its CTA. One that is cut by a range boundary leaves one
 // partial result (sum, maximum, denominator) per CTA that worked on it, and a second launch joins
@@ -47,7 +47,7 @@ struct AttentionArgs {
   int unit_rows;
   int tokens;                        // of a unit; 0 where a group is larger than a unit, and units cut tokens
   int token_shift;                   // its logarithm where it is a power of two, else -1
-  int unit_cost;
+  int unit_cost, pair_cost;          // on the line: of a unit, of a block for a unit of more than half the rows
   int ctas;                          // ranges
   // Partial results, in slots of some rows: maximum (scaled, base 2) and denominator [row], and the sum,
   // not divided by it, as [dim / 4][row][4], so that the threads of a warp, which own one row
@@ -121,10 +121,16 @@ __device__ __forceinline__ int unit_blocks(const AttentionArgs& a, const Sequenc
   return (visible_keys(a, s, min(last, s.n - 1)) + kKeys - 1) / kKeys;
 }
 
+__device__ __forceinline__ int block_cost(const AttentionArgs& a, const Sequence& s, int unit) {
+  return s.n - unit * a.tokens > a.tokens / 2 ? a.pair_cost : 1;
+}
+
 // Length of a unit on the line. A prompt's unit that sees no key is there all the same: somebody has
 // to write its zeros.
-__device__ __forceinline__ int unit_length(const AttentionArgs& a, int blocks) {
-  return blocks > 0 || a.kind == kPrompt ? blocks + a.unit_cost : 0;
+template <int kKeys>
+__device__ __forceinline__ int unit_length(const AttentionArgs& a, const Sequence& s, int unit) {
+  const int blocks = unit_blocks<kKeys>(a, s, unit);
+  return blocks > 0 || a.kind == kPrompt ? blocks * block_cost(a, s, unit) + a.unit_cost : 0;
 }
 
 // sum over i = 0 .. n - 1 of floor((a i + b) / m), for a, b >= 0: the whole multiples of m in a and b
@@ -150,18 +156,19 @@ static __device__ __noinline__ int64_t floor_sum(int n, int m, int a, int b) {
 template <int kKeys>
 __device__ __forceinline__ int length_before(const AttentionArgs& a, const Sequence& s, int units, int all) {
   if (units == 0) return 0;
-  if (a.kind == kShared || a.causal == 0) return units * unit_length(a, unit_blocks<kKeys>(a, s, 0));
+  const int regular = units < all ? units : all - 1;   // all but the last have all their rows
+  const int rest = units == all ? unit_length<kKeys>(a, s, all - 1) : 0;
+  if (a.kind == kShared || a.causal == 0) return (regular > 0 ? regular * unit_length<kKeys>(a, s, 0) : 0) + rest;
   if (a.tokens == 0) {
-    int sum = 0;
-    for (int t = 0; t < units; ++t) sum += unit_length(a, unit_blocks<kKeys>(a, s, t));
+    int sum = rest;
+    for (int t = 0; t < regular; ++t) sum += unit_length<kKeys>(a, s, t);
     return sum;
   }
   // Unit t holds whole tokens; but for the last of all, its last token sees c + tokens * (t + 1) keys.
   const int tokens = a.tokens, c = s.m - s.n;
-  const int regular = units < all ? units : all - 1;
   const int blind = c >= 0 ? 0 : min(-c / tokens, regular);   // units that see nothing
   const int n = regular - blind, b = c + tokens * (blind + 1) + kKeys - 1;
-  int sum = units * a.unit_cost;
+  int sum = 0;   // blocks
   if (a.token_shift < 0) {
     sum += static_cast<int>(floor_sum(n, kKeys, tokens, b));
   } else if (tokens >= kKeys) {
@@ -179,8 +186,7 @@ __device__ __forceinline__ int length_before(const AttentionArgs& a, const Seque
     };
     sum += static_cast<int>(below(first + n) - below(first));
   }
-  if (units == all) sum += unit_blocks<kKeys>(a, s, all - 1);
-  return sum;
+  return sum * a.pair_cost + regular * a.unit_cost + rest;
 }
 
 // ------------------------------------------------------------------------- finding a CTA's work
@@ -300,10 +306,10 @@ struct SegmentWalk {
 
   __device__ __forceinline__ bool next(Segment* out) {
     while (position < end) {
-      const int blocks = unit_blocks<kKeys>(a, seq, unit), length = unit_length(a, blocks);
+      const int blocks = unit_blocks<kKeys>(a, seq, unit), length = unit_length<kKeys>(a, seq, unit), cost = block_cost(a, seq, unit);
       const int from = offset, to = min(length, offset + end - position);
       const int unit_position = position - from;
-      Segment g{seq, head, unit, max(from - a.unit_cost, 0), max(to - a.unit_cost, 0), false, false, 0, 0};
+      Segment g{seq, head, unit, max(from - a.unit_cost, 0) / cost, max(to - a.unit_cost, 0) / cost, false, false, 0, 0};
       position += to - from;
       offset = to;
       if (to == length) {   // on to the next unit
@@ -319,9 +325,11 @@ struct SegmentWalk {
           }
         }
       }
-      // A range may end within what a unit costs beside its blocks, or hold only such a piece of it.
-      if (blocks > 0 ? g.block_end > g.block_begin : length > 0 && to == length) {
-        g.opens = g.block_begin == 0, g.whole = g.opens && g.block_end == blocks;
+      // A range may end within what a unit costs beside its blocks, or within a block; a block belongs
+      // to the range that holds its end. A range that holds only a piece of a block in the middle of
+      // a unit leaves an empty partial result: the join counts on one from every CTA on the way.
+      if (blocks > 0 ? g.block_end > 0 : length > 0 && to == length) {
+        g.opens = g.block_begin == 0, g.whole = g.opens && g.block_end == blocks;   // block_end > 0 or no blocks at all
         g.first_cta = blockIdx.x, g.last_cta = g.whole ? blockIdx.x : ranges.holder(unit_position + length - 1);
         *out = g;
         return true;

@@ -195,7 +195,7 @@ void plan_attention_simt(AttentionArgs* a, int sms) {
   const int tile = rows_per_sequence <= 16 ? 16 : 64;
   a->tokens = tile / a->group;
   a->unit_rows = a->tokens > 0 ? a->tokens * a->group : tile;
-  a->unit_cost = 1;
+  a->unit_cost = 1, a->pair_cost = 1;
   a->ctas = sms * (tile == 16 ? 3 : 2);
 }
 

@@ -9,8 +9,10 @@
 //
 // Two streams, each with its own group of four warps, O and S: the two row tiles of a unit of 256
 // rows, over the same blocks of 128 keys; or, where a unit has at most one tile of rows (a decoding
-// request, a short prompt), the even and the odd blocks for the same tile, joined at the end: thread r
-// of both groups of warps owns row r and may read both accumulators. Each stream has two S: while the
+// request, a short prompt), the first and the second 64 keys of each block for the same tile, joined
+// at the end: thread r of both groups of warps owns row r and may read both accumulators. (Even and odd
+// blocks instead kept two blocks at a time in the ring, whose next copies then came too late: a block
+// took as long as one of two tiles.) Each stream has two S: while the
 // warps work on one half block of 64 keys, the tensor pipe multiplies the P of the half before and
 // fills its place with the scores of the half after, so that neither waits for the other. (One S of
 // 128 keys per stream left the warps idle during the products: 4400 cycles per block of both streams
@@ -63,7 +65,7 @@ struct Smem {
 // What the roles need of a segment (attention.cuh), for a unit of whole tokens.
 struct SegmentEntry {
   int blocks;              // of keys; -1: no more segments
-  int pair;                // two row tiles over all blocks; else one tile, even and odd blocks
+  int pair;                // two row tiles over all keys; else one tile, its keys shared by the streams
   int q_row, tokens;       // the unit's first query row, and tokens from there to the sequence's end
   int k_row, batch, source, head;   // k_row: of the first block
   int keys, ahead;         // from the first block on: keys of the sequence; keys that token t of the unit sees
@@ -90,13 +92,8 @@ struct Shared {   // behind the tiles
 };
 constexpr int kEntryReaders = 1 + 2 + 8;
 
-// Half blocks of a stream: all of the segment's, or those of every other block.
-__device__ __forceinline__ int items_of(const SegmentEntry& e, int s) {
-  if (e.pair != 0) return e.halves;
-  const int own_blocks = (e.blocks + 1 - s) / 2;
-  const bool owns_last = e.blocks > 0 && ((e.blocks - 1) & 1) == s;
-  return 2 * own_blocks - (owns_last ? 2 * e.blocks - e.halves : 0);
-}
+// Half blocks of a stream: all of the segment's, or every other one.
+__device__ __forceinline__ int items_of(const SegmentEntry& e, int s) { return e.pair != 0 ? e.halves : (e.halves + 1 - s) / 2; }
 
 // A role's place in the ring of segments. Called by whole warps or by single threads.
 struct EntryReader {
@@ -254,82 +251,110 @@ __device__ __forceinline__ void copy_role(const UmmaAttentionArgs& p, uint8_t* s
 
 // One thread per stream.
 template <int kDim, bool kBf16>
-__device__ __forceinline__ void mma_role(const UmmaAttentionArgs& p, uint8_t* smem, Shared* b, uint32_t tmem, int s) {
+struct MmaIssuer {
   using S = Smem<kDim>;
-  const AttentionArgs& a = p.a;
-  constexpr uint32_t kIdescS = umma_idesc_f16(kTile, kHalf, kBf16, false, false);
-  const uint32_t idesc_o = umma_idesc_f16(kTile, (a.dim + 15) / 16 * 16, kBf16, false, true);
-  const int steps = (a.dim + 15) / 16;   // of 16 along the head dimension; what lies behind it reads as zero
-  const uint64_t q_desc[2] = {umma_smem_desc(smem_u32(smem), 16, 1024, kUmmaSwizzle128B),
-                              umma_smem_desc(smem_u32(smem) + S::kTileBytes, 16, 1024, kUmmaSwizzle128B)};
-  const uint64_t k_desc = umma_smem_desc(smem_u32(smem) + 2 * S::kTileBytes, 16, 1024, kUmmaSwizzle128B);
-  const uint64_t v_desc = umma_smem_desc(smem_u32(smem) + 2 * S::kTileBytes, S::kHalfBytes, 1024, kUmmaSwizzle128B);
-  const uint32_t s_at = tmem + kColS + s * kColStream, o_at = tmem + kColO + s * kColStream;
-  EntryReader reader{b};
-  uint32_t load = 0, segment = 0, own_segment = 0, p_phase = 0;   // p_phase: a bit per half
-  while (true) {
-    const SegmentEntry* entry = reader.wait();
-    const int blocks = entry->blocks;
-    const bool pair = entry->pair != 0;
-    const int items = items_of(*entry, s);
-    reader.release();
-    if (!reader.ok || blocks < 0) return;
-    if (blocks == 0) continue;
-    if (!mbar_wait(&b->q_full, segment & 1, kSiteAttention)) return;
-    ++segment;
-    const int step_blocks = pair ? 1 : 2, first = pair ? 0 : s;
-    // Both streams' threads count for a block of the ring; the one of a block that the other stream
-    // does not touch counts for it too.
-    const auto release = [&](uint32_t slot) {
-      if (!pair) mbar_arrive_relaxed(&b->empty[slot]);
-      umma_commit(&b->empty[slot]);
-    };
-    const auto arrived = [&](uint32_t at) { return mbar_wait(&b->full[at % S::kSlots], at / S::kSlots & 1, kSiteAttention); };
-    // Item j is half j & 1 of block first + (j >> 1) * step_blocks.
-    const auto load_of = [&](int j) { return load + 2 * (first + (j >> 1) * step_blocks); };
-    const auto scores = [&](int j) {   // K is there
-      const uint32_t slot = load_of(j) % S::kSlots, half = j & 1;
-      const uint64_t qd = q_desc[pair ? s : 0], kd = umma_desc_advance(k_desc, slot * S::kTileBytes + half * kHalf * 128);
-#pragma unroll
-      for (int step = 0; step < kDim / 16; ++step) {
-        if (step >= steps) break;
-        const uint32_t offset = (step >> 2) * S::kHalfBytes + (step & 3) * 32;
-        umma_f16(s_at + half * kColHalf, umma_desc_advance(qd, offset), umma_desc_advance(kd, offset), kIdescS, step > 0);
-      }
-      umma_commit(&b->s_full[s][half]);
-      if (half == 1 || j + 1 == items) release(slot);
-      if (j + 1 == items) umma_commit(&b->q_empty);
-    };
-    if (items == 0) {   // nothing for this stream
-      mbar_arrive(&b->q_empty);
-    } else {
-      if (!arrived(load_of(0))) return;
-      tcgen05_fence_after_sync();
-      scores(0);
-      if (items > 1) scores(1);
-      for (int j = 0; j < items; ++j) {
-        const uint32_t slot = (load_of(j) + 1) % S::kSlots, half = j & 1;
-        // A wait costs a few hundred cycles even when it is over already: everything but P is waited for
-        // before P, and what follows P is issued in one go.
-        if (half == 0 && (!arrived(load_of(j) + 1) || (j + 2 < items && !arrived(load_of(j + 2))))) return;
-        if (j == 0 && !mbar_wait(&b->o_empty[s], (own_segment & 1) ^ 1, kSiteAttention)) return;
-        if (!mbar_wait(&b->p_ready[s][half], p_phase >> half & 1, kSiteAttention)) return;
-        p_phase ^= 1u << half;
-        tcgen05_fence_after_sync();
-        const uint64_t vd = umma_desc_advance(v_desc, slot * S::kTileBytes + half * kHalf * 128);
-#pragma unroll
-        for (int step = 0; step < kHalf / 16; ++step)
-          umma_f16_tmem_a(o_at, s_at + half * kColHalf + step * 8, umma_desc_advance(vd, step * 2048), idesc_o, j > 0 || step > 0);
-        if (j + 2 < items) scores(j + 2);
-        if (j + 2 == items) umma_commit(&b->drained[s]);
-        if (j + 1 == items) umma_commit(&b->o_full[s]);
-        if (half == 1 || j + 1 == items) release(slot);
-      }
-      ++own_segment;
-    }
-    load += 2 * blocks;
+  static constexpr uint32_t kIdescS = umma_idesc_f16(kTile, kHalf, kBf16, false, false);
+  Shared* b;
+  int s, steps;   // stream; steps of 16 along the head dimension: what lies behind it reads as zero
+  uint32_t idesc_o, s_at, o_at;
+  uint64_t q_desc, k_desc, v_desc;
+  uint32_t load = 0, own_segment = 0, p_phase = 0;   // p_phase: a bit per S
+
+  __device__ __forceinline__ MmaIssuer(const AttentionArgs& a, uint8_t* smem, Shared* shared, uint32_t tmem, int stream) : b(shared), s(stream) {
+    steps = (a.dim + 15) / 16;
+    idesc_o = umma_idesc_f16(kTile, (a.dim + 15) / 16 * 16, kBf16, false, true);
+    s_at = tmem + kColS + s * kColStream, o_at = tmem + kColO + s * kColStream;
+    q_desc = umma_smem_desc(smem_u32(smem), 16, 1024, kUmmaSwizzle128B);
+    k_desc = umma_smem_desc(smem_u32(smem) + 2 * S::kTileBytes, 16, 1024, kUmmaSwizzle128B);
+    v_desc = umma_smem_desc(smem_u32(smem) + 2 * S::kTileBytes, S::kHalfBytes, 1024, kUmmaSwizzle128B);
   }
-}
+  __device__ __forceinline__ bool arrived(uint32_t at) const { return mbar_wait(&b->full[at % S::kSlots], at / S::kSlots & 1, kSiteAttention); }
+  __device__ __forceinline__ void release(uint32_t at) const { umma_commit(&b->empty[at % S::kSlots]); }   // both streams count for a block
+
+  // Item j is S buffer j & 1, over 64 keys of a block: both halves of it in turn, or (one tile) the
+  // stream's own.
+  template <bool kPair>
+  __device__ __forceinline__ uint32_t load_of(int j) const { return load + 2 * (kPair ? j >> 1 : j); }
+  template <bool kPair>
+  __device__ __forceinline__ uint32_t offset_of(uint32_t at, int j) const {   // of the item's keys or values in the ring
+    return at % S::kSlots * S::kTileBytes + (kPair ? j & 1 : s) * (kHalf * 128);
+  }
+  template <bool kPair>
+  __device__ __forceinline__ void scores(int j, int items) const {   // K is there
+    const uint64_t qd = kPair ? umma_desc_advance(q_desc, s * S::kTileBytes) : q_desc;
+    const uint64_t kd = umma_desc_advance(k_desc, offset_of<kPair>(load_of<kPair>(j), j));
+    const uint32_t at = s_at + (j & 1) * kColHalf;
+#pragma unroll
+    for (int step = 0; step < kDim / 16; ++step) {
+      if (step >= steps) break;
+      const uint32_t offset = (step >> 2) * S::kHalfBytes + (step & 3) * 32;
+      umma_f16(at, umma_desc_advance(qd, offset), umma_desc_advance(kd, offset), kIdescS, step > 0);
+    }
+    umma_commit(&b->s_full[s][j & 1]);
+    if (!kPair || (j & 1) == 1 || j + 1 == items) release(load_of<kPair>(j));
+    if (j + 1 == items) umma_commit(&b->q_empty);
+  }
+  template <bool kPair>
+  __device__ __forceinline__ bool segment(int items) {
+    if (!arrived(load)) return false;
+    tcgen05_fence_after_sync();
+    scores<kPair>(0, items);
+    if (items > 1) {
+      if (!kPair && !arrived(load_of<kPair>(1))) return false;
+      scores<kPair>(1, items);
+    }
+    for (int j = 0; j < items; ++j) {
+      const uint32_t buffer = j & 1, at = load_of<kPair>(j);
+      const bool opens = !kPair || (j & 1) == 0, more = j + 2 < items;
+      // A wait costs a few hundred cycles even when it is over already: what is due by now is waited for
+      // before P. (Not so the keys after next of a single tile: they are loaded only once the products
+      // before have freed a place in the ring.)
+      if (opens && !arrived(at + 1)) return false;
+      if (kPair && opens && more && !arrived(at + 2)) return false;
+      if (j == 0 && !mbar_wait(&b->o_empty[s], (own_segment & 1) ^ 1, kSiteAttention)) return false;
+      if (!mbar_wait(&b->p_ready[s][buffer], p_phase >> buffer & 1, kSiteAttention)) return false;
+      p_phase ^= 1u << buffer;
+      tcgen05_fence_after_sync();
+      const uint64_t vd = umma_desc_advance(v_desc, offset_of<kPair>(at + 1, j));
+#pragma unroll
+      for (int step = 0; step < kHalf / 16; ++step)
+        umma_f16_tmem_a(o_at, s_at + buffer * kColHalf + step * 8, umma_desc_advance(vd, step * 2048), idesc_o, j > 0 || step > 0);
+      if (!kPair) release(at + 1);
+      if (more) {
+        if (!kPair && !arrived(load_of<kPair>(j + 2))) return false;
+        scores<kPair>(j + 2, items);
+      }
+      if (j + 2 == items) umma_commit(&b->drained[s]);
+      if (j + 1 == items) umma_commit(&b->o_full[s]);
+      if (kPair && ((j & 1) == 1 || j + 1 == items)) release(at + 1);
+    }
+    ++own_segment;
+    return true;
+  }
+
+  __device__ __forceinline__ void run() {
+    EntryReader reader{b};
+    uint32_t segments = 0;
+    while (true) {
+      const SegmentEntry* entry = reader.wait();
+      const int blocks = entry->blocks, items = items_of(*entry, s);
+      const bool pair = entry->pair != 0;
+      reader.release();
+      if (!reader.ok || blocks < 0) return;
+      if (blocks == 0) continue;
+      if (!mbar_wait(&b->q_full, segments++ & 1, kSiteAttention)) return;
+      if (items == 0) mbar_arrive(&b->q_empty);
+      else if (!(pair ? segment<true>(items) : segment<false>(items))) return;
+      if (!pair && items < blocks) {   // the last block has no keys for this stream
+        for (uint32_t at = load + 2 * blocks - 2; at != load + 2 * blocks; ++at) {
+          if (!arrived(at)) return;
+          mbar_arrive(&b->empty[at % S::kSlots]);
+        }
+      }
+      load += 2 * blocks;
+    }
+  }
+};
 
 // ------------------------------------------------------------------------------------ softmax
 
@@ -339,8 +364,10 @@ struct RowState {
 };
 
 // One half block. `settled` waits until the products of the half before are in O.
+// A NaN among the scores that a row sees, or +infinity, whose difference from itself is one, makes its
+// maximum NaN and with it everything that follows.
 template <bool kBf16, bool kMasked, class Settled>
-__device__ __forceinline__ void softmax_half(uint32_t s_at, uint32_t o_at, int chunks, int seen, float scale, bool first, RowState* row,
+__device__ __forceinline__ void softmax_half(uint32_t s_at, uint32_t o_at, int chunks, bool live, int seen, float scale, bool first, RowState* row,
                                              const Settled& settled) {
   float x[kHalf];
   tmem_ld_32x32(s_at, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
@@ -356,13 +383,15 @@ __device__ __forceinline__ void softmax_half(uint32_t s_at, uint32_t o_at, int c
 #pragma unroll
   for (int i = 0; i < kHalf; i += 8) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) top[j] = max3(top[j], x[i + j], x[i + 4 + j]);
+    for (int j = 0; j < 4; ++j) top[j] = max3_nan(top[j], x[i + j], x[i + 4 + j]);
   }
-  const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+  float m = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]) * scale;
+  if (m == -kMinusInf) m = __int_as_float(0x7fffffff);
+  if (!live) m = 0.f;   // lanes without a row hold anything; they must not ask for rescaling
   if (first) {
     row->m = m;
   } else {
-    const bool grown = m > row->m + kLazy;
+    const bool grown = !(m <= row->m + kLazy);   // or NaN
     if (__any_sync(0xffffffffu, grown)) {
       const float next = grown ? m : row->m;
       const float keep = grown ? exp2_fast(row->m - next) : 1.f;
@@ -445,7 +474,7 @@ __device__ __forceinline__ void softmax_role(const UmmaAttentionArgs& p, Shared*
     const int token0 = pair && s == 1 ? tile_tokens : 0;   // of the tile within the unit
     const int q_row = entry->q_row + token0, head = entry->head * a.group;
     const int64_t slot = entry->slot;
-    const int items = ok ? items_of(*entry, s) : 0;
+    const int items = ok ? items_of(*entry, s) : 0, halves = entry->halves;
     const int pitch = entry->pitch, slot_row = (pair && s == 1 ? tile_rows : 0) + r;
     __syncwarp();
     if (lane == 0) reader.release();
@@ -462,7 +491,7 @@ __device__ __forceinline__ void softmax_role(const UmmaAttentionArgs& p, Shared*
     const int seen_by_all = clamp_int(ahead + token0 + token_warp, 0, keys);
     for (int j = 0; j < items; ++j) {
       const uint32_t half = j & 1;
-      const int key0 = (pair ? j : 4 * (j >> 1) + 2 * s + (j & 1)) * kHalf;
+      const int key0 = (pair ? j : 2 * j + s) * kHalf;
       ok = __all_sync(0xffffffffu, ok && mbar_wait(&b->s_full[s][half], s_phase >> half & 1, kSiteAttention));
       s_phase ^= 1u << half;
       if (ok && warp_live) {
@@ -476,8 +505,8 @@ __device__ __forceinline__ void softmax_role(const UmmaAttentionArgs& p, Shared*
           tcgen05_fence_after_sync();
         };
         const uint32_t at = s_at + half * kColHalf;
-        if (key0 + kHalf <= seen_by_all) softmax_half<kBf16, false>(at, o_at, chunks, 0, a.scale_log2, j == 0, &row, settled);
-        else softmax_half<kBf16, true>(at, o_at, chunks, seen - key0, a.scale_log2, j == 0, &row, settled);
+        if (key0 + kHalf <= seen_by_all) softmax_half<kBf16, false>(at, o_at, chunks, live, 0, a.scale_log2, j == 0, &row, settled);
+        else softmax_half<kBf16, true>(at, o_at, chunks, live, seen - key0, a.scale_log2, j == 0, &row, settled);
         tcgen05_fence_before_sync();
       }
       __syncwarp();
@@ -486,7 +515,7 @@ __device__ __forceinline__ void softmax_role(const UmmaAttentionArgs& p, Shared*
     if (items > 1) drain_phase ^= 1;
     // Rows of one tile that two streams worked on: the same thread of both warp groups owns them, and
     // each finishes every other 32 columns.
-    const bool joined = !pair && blocks > 1;
+    const bool joined = !pair && halves > 1;
     float mine = 1.f, other = 0.f, total = row.l, base = row.m;
     if (joined) {
       b->exchange[s][r] = make_float2(row.m, row.l);
@@ -614,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_umma_kernel(const __gri
   } else {
     registers_lower<kOtherRegisters>();
     if (warp == 8 && lane == 0) copy_role<kDim>(p, smem, &b);
-    if ((warp == 9 || warp == 10) && lane == 0) mma_role<kDim, kBf16>(p, smem, &b, tmem, warp - 9);
+    if ((warp == 9 || warp == 10) && lane == 0) MmaIssuer<kDim, kBf16>(p.a, smem, &b, tmem, warp - 9).run();
     if (warp == 11) segment_role<kDim>(p, start, smem, &b);
   }
   __syncwarp();
@@ -659,7 +688,7 @@ void plan_attention_umma(AttentionArgs* a, int sms) {
   // Tiles hold whole tokens: a copy brings (dim, group, tokens) boxes.
   a->tokens = 2 * (kTile / a->group);
   a->unit_rows = a->tokens * a->group;
-  a->unit_cost = 1;
+  a->unit_cost = 3, a->pair_cost = 2;   // a block of one tile takes about 1.2 us, a unit beside its blocks 2 to 3
   a->ctas = sms;
 }
 
