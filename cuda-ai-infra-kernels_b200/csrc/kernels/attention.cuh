@@ -152,9 +152,10 @@ static __device__ __noinline__ int64_t floor_sum(int n, int m, int a, int b) {
 }
 
 // Length of the first `units` of the `all` units of one key head of the sequence. The launcher has made
-// sure that the whole line fits 32 bits.
+// sure that the whole line fits 32 bits. Not inlined: a CTA calls it three or four times as it starts,
+// when every instruction has to be fetched before it runs.
 template <int kKeys>
-__device__ __forceinline__ int length_before(const AttentionArgs& a, const Sequence& s, int units, int all) {
+__device__ __noinline__ int length_before(const AttentionArgs& a, const Sequence& s, int units, int all) {
   if (units == 0) return 0;
   const int regular = units < all ? units : all - 1;   // all but the last have all their rows
   const int rest = units == all ? unit_length<kKeys>(a, s, all - 1) : 0;

@@ -4,7 +4,10 @@
 // Bound by HBM: the logits are read once and written once. A CTA owns a stretch of one row's
 // vocabulary and counts, in shared memory, the occurrences of its tokens in the row's history (it
 // reads the whole history, which the row's other CTAs read too, from L2; integer atomics, so the
-// order does not matter). Counting per stretch needs no workspace and no second launch.
+// order does not matter). Counting per stretch needs no workspace and no second launch. Tokens are
+// listed as they are first met. The pass over the stretch only copies and masks; the listed tokens
+// are then computed again. (Looking the counters up in the pass itself sent nearly every warp through
+// the penalties' divisions for a few of its 256 tokens: 67 us instead of HBM's 17 for 256 rows.)
 //
 // A row of odd length starts anywhere in a 16-byte granule. Stretches are therefore cut in the
 // granules of the array, not of the row: position e of the stretch space of row r is token
@@ -13,6 +16,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "host_common.h"
 #include "ptx_sm100.cuh"
 
@@ -20,7 +25,6 @@ namespace b200 {
 namespace {
 
 constexpr int kLogitsThreads = 256;
-constexpr uint32_t kInPrompt = 1u << 31;   // the other bits count occurrences in the output
 
 struct LogitsArgs {
   b200_logits_problem q;
@@ -40,46 +44,99 @@ struct RowPenalties {
   float repetition, frequency, presence;
 };
 
-__device__ __forceinline__ float penalised(float x, uint32_t count, const RowPenalties& p) {
+__device__ __forceinline__ float penalised(float x, uint32_t count, uint32_t seen_bit, const RowPenalties& p) {
   if (count == 0) return x;
   x = x > 0.f ? x / p.repetition : x * p.repetition;
-  const uint32_t made = count & ~kInPrompt;
+  const uint32_t made = count & ~seen_bit;
   return made == 0 ? x : x - (p.frequency * static_cast<float>(made) + p.presence);
 }
 
+// Counters of a stretch: 32 bits per position, or 16 where the output is too short to overflow 15 (twice
+// the stretch in the same shared memory, and half as many readings of the history).
+template <bool kNarrow>
+struct Counters {
+  static constexpr uint32_t kSeen = kNarrow ? 1u << 15 : 1u << 31;   // in the prompt; the other bits count the output
+  uint32_t* words;
+  // Both say whether the token is met for the first time.
+  __device__ __forceinline__ bool prompt(int at) const {
+    if (kNarrow) return (atomicOr(words + (at >> 1), kSeen << (16 * (at & 1))) >> (16 * (at & 1)) & 0xffffu) == 0;
+    return atomicOr(words + at, kSeen) == 0;
+  }
+  __device__ __forceinline__ bool output(int at) const {
+    if (kNarrow) return (atomicAdd(words + (at >> 1), 1u << (16 * (at & 1))) >> (16 * (at & 1)) & 0xffffu) == 0;
+    return atomicAdd(words + at, 1u) == 0;
+  }
+  __device__ __forceinline__ uint32_t operator[](int at) const {
+    return kNarrow ? words[at >> 1] >> (16 * (at & 1)) & 0xffffu : words[at];
+  }
+};
+
+// Minus infinity in the granule's elements whose bit is clear.
+template <typename T>
+__device__ __forceinline__ uint4 masked(uint4 v, uint32_t bits) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+  if constexpr (sizeof(T) == 2) {
+    constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {   // a bit moved to the top of a byte, whose sign fills half a word
+      uint32_t keep;
+      asm("prmt.b32 %0, %1, %2, 0xcc88;" : "=r"(keep) : "r"(bits << 7 >> 2 * i), "r"(bits << 6 >> 2 * i));
+      w[i] = (w[i] & keep) | (kInf & ~keep);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if ((bits >> i & 1) == 0) w[i] = 0xff800000u;
+  }
+  return v;
+}
+
 // Counts the tokens of one history that fall into [first, first + positions).
+template <bool kNarrow, bool kPrompt>
 __device__ __forceinline__ void count_tokens(const int32_t* tokens, int64_t length, int64_t first, int positions, int64_t vocab,
-                                             uint32_t* counts, bool prompt) {
-  for (int64_t i = threadIdx.x; i < length; i += kLogitsThreads) {
-    const int64_t token = __ldg(tokens + i);
-    const int64_t at = token - first;
-    if (token >= 0 && token < vocab && at >= 0 && at < positions) {
-      if (prompt) atomicOr(counts + at, kInPrompt);
-      else atomicAdd(counts + at, 1u);
+                                             const Counters<kNarrow>& counts, uint16_t* list, int* listed) {
+  // Tokens of the stretch that the vocabulary has, as an unsigned range.
+  const int32_t low = static_cast<int32_t>(first > 0 ? first : 0);
+  const uint32_t span = static_cast<uint32_t>((first + positions < vocab ? first + positions : vocab) - low);
+  constexpr int kAhead = 8;
+  for (int64_t i = threadIdx.x; i < length; i += kAhead * kLogitsThreads) {
+    int32_t token[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) token[j] = i + j * kLogitsThreads < length ? __ldg(tokens + i + j * kLogitsThreads) : -1;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (token[j] >= 0 && static_cast<uint32_t>(token[j] - low) < span) {
+        const int at = static_cast<int>(token[j] - first);
+        if (kPrompt ? counts.prompt(at) : counts.output(at)) list[atomicAdd(listed, 1)] = static_cast<uint16_t>(at);
+      }
     }
   }
 }
 
-template <typename T>
+template <typename T, bool kNarrow>
 __global__ void __launch_bounds__(kLogitsThreads) logits_kernel(const LogitsArgs a) {
-  extern __shared__ __align__(16) uint32_t counts[];
+  extern __shared__ __align__(16) uint32_t words[];
   constexpr int kVec = 16 / sizeof(T);
   const b200_logits_problem& q = a.q;
+  __shared__ int listed;
+  const Counters<kNarrow> counts{words};
+  uint16_t* list = reinterpret_cast<uint16_t*>(words + a.stretch / (kNarrow ? 2 : 1));
+  constexpr uint32_t kSeen = Counters<kNarrow>::kSeen;
   grid_launch_dependents();
-  for (int i = threadIdx.x; i < a.stretch; i += kLogitsThreads) counts[i] = 0;
+  if (threadIdx.x == 0) listed = 0;
+  for (int i = threadIdx.x; i < a.stretch / (kNarrow ? 8 : 4); i += kLogitsThreads) reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
   grid_dependency_wait();
   const int64_t row = blockIdx.x / a.stretches;
   const int64_t lead = (row * q.vocab) % kVec;
   const int64_t first = static_cast<int64_t>(blockIdx.x % a.stretches) * a.stretch - lead;   // token of position 0; may be negative
+  if (first >= q.vocab) return;
   RowPenalties p{1.f, 0.f, 0.f};
   if (q.repetition != nullptr) p.repetition = q.repetition[row];
   if (q.frequency != nullptr) p.frequency = q.frequency[row];
   if (q.presence != nullptr) p.presence = q.presence[row];
-  if (q.prompt_tokens != nullptr) count_tokens(q.prompt_tokens + row * q.prompt_length, q.prompt_length, first, a.stretch, q.vocab, counts, true);
-  if (q.output_tokens != nullptr) count_tokens(q.output_tokens + row * q.output_length, q.output_length, first, a.stretch, q.vocab, counts, false);
-  __syncthreads();
-
+  if (q.prompt_tokens != nullptr) count_tokens<kNarrow, true>(q.prompt_tokens + row * q.prompt_length, q.prompt_length, first, a.stretch, q.vocab, counts, list, &listed);
+  if (q.output_tokens != nullptr) count_tokens<kNarrow, false>(q.output_tokens + row * q.output_length, q.output_length, first, a.stretch, q.vocab, counts, list, &listed);
   const T* x = static_cast<const T*>(q.logits) + row * q.vocab;
   T* y = static_cast<T*>(q.out) + row * q.vocab;
   const uint32_t* allowed = q.allowed == nullptr ? nullptr : reinterpret_cast<const uint32_t*>(q.allowed) + row * q.allowed_stride;
@@ -87,38 +144,80 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_kernel(const LogitsArgs
     const bool keep = allowed == nullptr || (__ldg(allowed + token / 32) >> (token % 32) & 1u) != 0;
     return from_float<T>(keep ? v : __int_as_float(0xff800000));
   };
-  for (int e = threadIdx.x * kVec; e < a.stretch; e += kLogitsThreads * kVec) {
-    const int64_t token = first + e;
-    if (token >= q.vocab) break;
-    for (int i = 0; i < kVec; ++i) {
-      const int64_t t = token + i;
-      if (t >= 0 && t < q.vocab) y[t] = finish(t, penalised(to_float(x[t]), counts[e + i], p));
+  // Whole granules, four of them on their way per thread.
+  constexpr int kAhead = 4;
+  constexpr uint32_t kAll = (1u << kVec) - 1;
+  for (int e0 = threadIdx.x * kVec; e0 < a.stretch; e0 += kAhead * kLogitsThreads * kVec) {
+    uint4 v[kAhead];
+    uint32_t bits[kAhead];
+    bool whole[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int e = e0 + j * kLogitsThreads * kVec;
+      const int64_t token = first + e;
+      whole[j] = e < a.stretch && token >= 0 && token + kVec <= q.vocab;
+      bits[j] = kAll;
+      if (whole[j]) {
+        v[j] = __ldcs(reinterpret_cast<const uint4*>(x + token));
+        if (allowed != nullptr) {   // kVec bits from bit `token` on, out of one word or two
+          const uint32_t at = static_cast<uint32_t>(token) / 32, shift = static_cast<uint32_t>(token) % 32;
+          const uint32_t lo = __ldg(allowed + at), hi = shift + kVec > 32 ? __ldg(allowed + at + 1) : 0;
+          bits[j] = __funnelshift_r(lo, hi, shift) & kAll;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int e = e0 + j * kLogitsThreads * kVec;
+      const int64_t token = first + e;
+      if (whole[j]) {
+        __stcs(reinterpret_cast<uint4*>(y + token), bits[j] == kAll ? v[j] : masked<T>(v[j], bits[j]));
+      } else if (e < a.stretch) {   // shared with the row before or behind
+        for (int i = 0; i < kVec; ++i) {
+          const int64_t t = token + i;
+          if (t >= 0 && t < q.vocab) y[t] = finish(t, to_float(x[t]));
+        }
+      }
     }
   }
+  __syncthreads();   // the counters are complete, and the stretch is stored
+  for (int i = threadIdx.x; i < listed; i += kLogitsThreads) {
+    const int at = list[i];
+    const int64_t token = first + at;
+    y[token] = finish(token, penalised(to_float(x[token]), counts[at], kSeen, p));
+  }
   if (q.bias_ids == nullptr) return;
-  // Biased tokens are computed again from the start, after the pass above has stored them. The
-  // first entry of a token adds up the values of all its entries, in their order.
+  // Biased tokens are computed once more from the start. The first entry of a token adds up the values
+  // of all its entries, in their order.
   __syncthreads();
   const int32_t* ids = q.bias_ids + row * q.bias_length;
   const float* values = q.bias_values + row * q.bias_length;
-  for (int64_t i = threadIdx.x; i < q.bias_length; i += kLogitsThreads) {
-    const int64_t token = ids[i];
+  const int lane = threadIdx.x & 31;
+  for (int64_t i = threadIdx.x >> 5; i < q.bias_length; i += kLogitsThreads / 32) {   // a warp per entry
+    const int64_t token = __ldg(ids + i);
     const int64_t at = token - first;
     if (token < 0 || token >= q.vocab || at < 0 || at >= a.stretch) continue;
     bool earlier = false;
-    for (int64_t j = 0; j < i; ++j) earlier |= ids[j] == token;
-    if (earlier) continue;
     float bias = 0.f;
-    for (int64_t j = i; j < q.bias_length; ++j) bias += ids[j] == token ? values[j] : 0.f;
-    y[token] = finish(token, penalised(to_float(x[token]), counts[at], p) + bias);
+    for (int64_t j0 = 0; j0 < q.bias_length && !earlier; j0 += 32) {
+      const int64_t j = j0 + lane;
+      uint32_t same = __ballot_sync(0xffffffffu, j < q.bias_length && __ldg(ids + j) == token);
+      for (; same != 0; same &= same - 1) {
+        const int64_t k = j0 + __ffs(same) - 1;
+        earlier |= k < i;
+        bias += __ldg(values + k);
+      }
+    }
+    if (!earlier && lane == 0) y[token] = finish(token, penalised(to_float(x[token]), counts[static_cast<int>(at)], kSeen, p) + bias);
   }
 }
 
-template <typename T>
-int launch_logits(const b200_logits_problem& q, cudaStream_t s) {
+template <typename T, bool kNarrow>
+int launch_counted(const b200_logits_problem& q, cudaStream_t s) {
   constexpr int kVec = 16 / static_cast<int>(sizeof(T));
-  LogitsArgs a{q, 8192, 0};
-  // A short stretch for few rows: at least two CTAs per SM where the vocabulary allows it.
+  // 32 KiB of counters: seven CTAs per SM. A short stretch for few rows: at least two CTAs per SM where
+  // the vocabulary allows it.
+  LogitsArgs a{q, kNarrow ? 16384 : 8192, 0};
   const int64_t wanted = 2 * static_cast<int64_t>(sm_count());
   while (a.stretch > 1024 && q.rows * ((q.vocab + a.stretch - 1) / a.stretch) < wanted) a.stretch /= 2;
   a.stretches = static_cast<int>((q.vocab + kVec - 1 + a.stretch - 1) / a.stretch);
@@ -127,13 +226,21 @@ int launch_logits(const b200_logits_problem& q, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(kLogitsThreads);
-  cfg.dynamicSmemBytes = a.stretch * sizeof(uint32_t);
+  // Counters, and the list of the stretch's tokens that are in the history.
+  const int64_t history = (q.prompt_tokens != nullptr ? q.prompt_length : 0) + (q.output_tokens != nullptr ? q.output_length : 0);
+  cfg.dynamicSmemBytes = a.stretch * (kNarrow ? sizeof(uint16_t) : sizeof(uint32_t)) + sizeof(uint16_t) * (history < a.stretch ? history : a.stretch);
   cfg.stream = s;
+  if (!ensure_dynamic_smem<logits_kernel<T, kNarrow>, 64 * 1024>()) return B200_ERR_LAUNCH_FAILED;
   const GemmLaunchAttributes attrs = gemm_launch_attributes(1);
   cfg.attrs = const_cast<cudaLaunchAttribute*>(attrs.list);
   cfg.numAttrs = attrs.count;
-  if (cudaLaunchKernelEx(&cfg, logits_kernel<T>, a) != cudaSuccess) return launch_failed();
+  if (cudaLaunchKernelEx(&cfg, logits_kernel<T, kNarrow>, a) != cudaSuccess) return launch_failed();
   return launch_status();
+}
+
+template <typename T>
+int launch_logits(const b200_logits_problem& q, cudaStream_t s) {
+  return q.output_length < (1 << 15) ? launch_counted<T, true>(q, s) : launch_counted<T, false>(q, s);
 }
 
 }  // namespace

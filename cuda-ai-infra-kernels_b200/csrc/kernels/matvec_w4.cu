@@ -14,11 +14,20 @@
 // subtracting 1024 + zero or 128 + zero leaves c - zero, exact. Each step of K lies inside one group:
 // its FP32 product is multiplied by the group's scale when it is added to the running sum.
 //
+// What it measured: one BF16 row by 28672 x 8192 (117 MB of weights) 44.8 us, FP16 42.1, against 18.5 for
+// the weights at the copy bandwidth: issue slots 58 % busy, the integer pipe 61 %, HBM 30 %. Four
+// things that did not help, all timed side by side: 32 rows per warp (x shared, half the warps: 51.5);
+// more warps by fewer registers (51.6 with five CTAs per SM instead of four, 55.3 with six); the warps
+// side by side along K instead of in ranges (45.6); and integer matrix instructions on the raw codes with
+// x in signed 8-bit digits, a third of the instructions (62).
+//
 // FP32 x is written as the sum of three BF16 numbers (8 + 8 + 8 bits, by truncation: exact), which take
 // three columns of the instruction and are added up at the end, so that products and sums are as
 // accurate as FP32 arithmetic.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "host_common.h"
 #include "ptx_sm100.cuh"
@@ -59,6 +68,37 @@ template <> struct Pair<__nv_bfloat16> {
   }
 };
 template <> struct Pair<float> : Pair<__nv_bfloat16> {};   // FP32 x travels as three BF16 columns
+
+// The eight codes of a word, less their zero: pairs (0,4), (1,5), (2,6), (3,7). These are most of the
+// kernel's instructions, so there are as few as the type allows:
+// the ten mantissa bits of FP16 hold a code in bits 4..7 as well, sixteen times too large, which the
+// subtraction's multiply-add takes back for nothing; the seven of BF16 do not.
+struct ZeroPair {
+  uint32_t low, high;   // what to subtract from a code in bits 0..3, and in bits 4..7
+};
+template <typename T>
+__device__ __forceinline__ ZeroPair zero_pair(uint32_t z) {
+  const uint32_t twice = z | z << 16;
+  // 1024 + z as it is; a code in bits 4..7 reads 1024 + 16 c and is divided by 16, which leaves 64 + c.
+  return {Pair<T>::kBase | twice, 0xd400d400u | twice << 4};   // FP16: -(64 + z)
+}
+template <typename T>
+__device__ __forceinline__ void decode(uint32_t (&out)[4], uint32_t w, const ZeroPair& zero) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const uint32_t upper = w >> 8;
+    const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00));
+    const auto high = [&](uint32_t v) {
+      const uint32_t c = (v & 0x00f000f0u) | Pair<T>::kBase;
+      const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&c), sixteenth, *reinterpret_cast<const __half2*>(&zero.high));
+      return *reinterpret_cast<const uint32_t*>(&r);
+    };
+    out[0] = Pair<T>::sub((w & 0x000f000fu) | Pair<T>::kBase, zero.low), out[1] = high(w);
+    out[2] = Pair<T>::sub((upper & 0x000f000fu) | Pair<T>::kBase, zero.low), out[3] = high(upper);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] = Pair<T>::sub((w >> (4 * j) & 0x000f000fu) | Pair<T>::kBase, zero.low);
+  }
+}
 
 template <int kBytes> struct Packed;
 template <> struct Packed<16> {
@@ -128,49 +168,60 @@ __global__ void __launch_bounds__(kWarps * 32) matvec_w4_kernel(const W4Args a) 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quad = lane >> 2, t = lane & 3;
   const int row0 = blockIdx.x * 16;
-  const int groups = q.k / q.group;
-  // Rows behind the last are read as the last one and not stored.
-  const int64_t r[2] = {min(row0 + quad, q.n - 1), min(row0 + quad + 8, q.n - 1)};
+  const int groups = q.k / q.group, group_steps = q.group / kStep;
   const int steps = q.k / kStep;
   const int begin = static_cast<int>(static_cast<int64_t>(steps) * warp / kWarps), end = static_cast<int>(static_cast<int64_t>(steps) * (warp + 1) / kWarps);
-  const uint8_t* w0 = q.qweight + r[0] * (q.k / 2) + t * kBytes;
-  const uint8_t* w1 = q.qweight + r[1] * (q.k / 2) + t * kBytes;
+  // This thread's two weight rows. Rows behind the last are read as the last one and not stored.
+  const uint8_t* w[2];
+  int64_t at[2];   // of the group's scale and zero
+  int group = begin / group_steps, left = (group + 1) * group_steps - begin;   // steps left in the group
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t r = min(row0 + 8 * i + quad, q.n - 1);
+    w[i] = q.qweight + r * (q.k / 2) + t * kBytes + static_cast<int64_t>(begin) * (kStep / 2);
+    at[i] = r * groups + group;
+  }
 
   float total[kTiles][4] = {};
-#pragma unroll 4
+  float scale[2];
+  ZeroPair zero[2];
+  bool fresh = true;
+#pragma unroll 2
   for (int s = begin; s < end; ++s) {
-    Packed<kBytes> p0, p1;
-    p0.load(w0 + static_cast<int64_t>(s) * (kStep / 2));
-    p1.load(w1 + static_cast<int64_t>(s) * (kStep / 2));
-    const int group = s * kStep / q.group;
-    const int64_t at0 = r[0] * groups + group, at1 = r[1] * groups + group;
-    const float scale0 = scale_at(q.scales, q.scale_dtype, at0), scale1 = scale_at(q.scales, q.scale_dtype, at1);
-    const uint32_t z0 = q.zeros == nullptr ? 8u : __ldg(q.zeros + at0) & 15u, z1 = q.zeros == nullptr ? 8u : __ldg(q.zeros + at1) & 15u;
-    const uint32_t base0 = Pair<T>::kBase | z0 | z0 << 16, base1 = Pair<T>::kBase | z1 | z1 << 16;
+    Packed<kBytes> p[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) p[i].load(w[i]), w[i] += kStep / 2;
+    if (fresh) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        scale[i] = scale_at(q.scales, q.scale_dtype, at[i]);
+        zero[i] = zero_pair<T>(q.zeros == nullptr ? 8u : __ldg(q.zeros + at[i]) & 15u);
+        ++at[i];
+      }
+    }
+    fresh = --left == 0;
+    if (fresh) left = group_steps;
     float acc[kTiles][4] = {};
 #pragma unroll
     for (int i = 0; i < kBytes / 4; ++i) {
-      uint32_t m0[4], m1[4];
+      uint32_t m[2][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        m0[j] = Pair<T>::sub((p0.w[i] >> (4 * j) & 0x000f000fu) | Pair<T>::kBase, base0);
-        m1[j] = Pair<T>::sub((p1.w[i] >> (4 * j) & 0x000f000fu) | Pair<T>::kBase, base1);
-      }
+      for (int r = 0; r < 2; ++r) decode<T>(m[r], p[r].w[i], zero[r]);
+      const uint32_t first[4] = {m[0][0], m[1][0], m[0][1], m[1][1]}, second[4] = {m[0][2], m[1][2], m[0][3], m[1][3]};
       const int64_t k = static_cast<int64_t>(s) * kStep + t * 2 * kBytes + i * 8;
 #pragma unroll
       for (int c = 0; c < kTiles; ++c) {
         const int column = c * 8 + quad;
         uint32_t x[4] = {0, 0, 0, 0};
         if (column < q.rows * kParts) load_pairs<T>(x, static_cast<const T*>(q.x) + static_cast<int64_t>(column / kParts) * q.k + k, column % kParts);
-        const uint32_t first[4] = {m0[0], m1[0], m0[1], m1[1]}, second[4] = {m0[2], m1[2], m0[3], m1[3]};
         Pair<T>::mma(acc[c], first, x[0], x[1]);
         Pair<T>::mma(acc[c], second, x[2], x[3]);
       }
     }
 #pragma unroll
     for (int c = 0; c < kTiles; ++c) {
-      total[c][0] += scale0 * acc[c][0], total[c][1] += scale0 * acc[c][1];
-      total[c][2] += scale1 * acc[c][2], total[c][3] += scale1 * acc[c][3];
+      total[c][0] += scale[0] * acc[c][0], total[c][1] += scale[0] * acc[c][1];
+      total[c][2] += scale[1] * acc[c][2], total[c][3] += scale[1] * acc[c][3];
     }
   }
 #pragma unroll
@@ -183,9 +234,9 @@ __global__ void __launch_bounds__(kWarps * 32) matvec_w4_kernel(const W4Args a) 
     const int n = i % 16, m = i / 16;
     if (row0 + n >= q.n) continue;
     float sum = 0.f;
-    for (int w = 0; w < kWarps; ++w)
+    for (int v = 0; v < kWarps; ++v)
 #pragma unroll
-      for (int part = 0; part < kParts; ++part) sum += sums[w][n][m * kParts + part];
+      for (int part = 0; part < kParts; ++part) sum += sums[v][n][m * kParts + part];
     store_out(static_cast<T*>(q.y) + static_cast<int64_t>(m) * q.n + row0 + n, sum);
   }
 }
