@@ -135,9 +135,22 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_kernel(const LogitsArgs
   if (q.repetition != nullptr) p.repetition = q.repetition[row];
   if (q.frequency != nullptr) p.frequency = q.frequency[row];
   if (q.presence != nullptr) p.presence = q.presence[row];
+  // The thread's bias entry, on its way from the start: what it needs comes from far away, one after the other.
+  __shared__ int bias_ids[kLogitsThreads];
+  __shared__ float bias_values[kLogitsThreads];
+  const T* x = static_cast<const T*>(q.logits) + row * q.vocab;
+  int bias_id = -1;
+  float bias_value = 0.f, bias_logit = 0.f;
+  const auto fetch_bias = [&](int64_t from) {
+    const int64_t i = from + threadIdx.x;
+    bias_id = q.bias_ids != nullptr && i < q.bias_length ? __ldg(q.bias_ids + row * q.bias_length + i) : -1;
+    if (bias_id < 0 || bias_id >= q.vocab) bias_id = -1;
+    if (bias_id >= 0) bias_value = __ldg(q.bias_values + row * q.bias_length + i);
+    if (bias_id >= first && bias_id >= 0 && bias_id < first + a.stretch) bias_logit = to_float(x[bias_id]);
+  };
+  fetch_bias(0);
   if (q.prompt_tokens != nullptr) count_tokens<kNarrow, true>(q.prompt_tokens + row * q.prompt_length, q.prompt_length, first, a.stretch, q.vocab, counts, list, &listed);
   if (q.output_tokens != nullptr) count_tokens<kNarrow, false>(q.output_tokens + row * q.output_length, q.output_length, first, a.stretch, q.vocab, counts, list, &listed);
-  const T* x = static_cast<const T*>(q.logits) + row * q.vocab;
   T* y = static_cast<T*>(q.out) + row * q.vocab;
   const uint32_t* allowed = q.allowed == nullptr ? nullptr : reinterpret_cast<const uint32_t*>(q.allowed) + row * q.allowed_stride;
   const auto finish = [&](int64_t token, float v) {
@@ -181,34 +194,41 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_kernel(const LogitsArgs
     }
   }
   __syncthreads();   // the counters are complete, and the stretch is stored
-  for (int i = threadIdx.x; i < listed; i += kLogitsThreads) {
-    const int at = list[i];
-    const int64_t token = first + at;
-    y[token] = finish(token, penalised(to_float(x[token]), counts[at], kSeen, p));
+  for (int i = threadIdx.x; i < listed; i += kAhead * kLogitsThreads) {
+    float value[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)   // all on their way before the first store
+      if (i + j * kLogitsThreads < listed) value[j] = to_float(x[first + list[i + j * kLogitsThreads]]);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (i + j * kLogitsThreads >= listed) break;
+      const int at = list[i + j * kLogitsThreads];
+      y[first + at] = finish(first + at, penalised(value[j], counts[at], kSeen, p));
+    }
   }
   if (q.bias_ids == nullptr) return;
   // Biased tokens are computed once more from the start. The first entry of a token adds up the values
-  // of all its entries, in their order.
-  __syncthreads();
-  const int32_t* ids = q.bias_ids + row * q.bias_length;
-  const float* values = q.bias_values + row * q.bias_length;
-  const int lane = threadIdx.x & 31;
-  for (int64_t i = threadIdx.x >> 5; i < q.bias_length; i += kLogitsThreads / 32) {   // a warp per entry
-    const int64_t token = __ldg(ids + i);
-    const int64_t at = token - first;
-    if (token < 0 || token >= q.vocab || at < 0 || at >= a.stretch) continue;
-    bool earlier = false;
-    float bias = 0.f;
-    for (int64_t j0 = 0; j0 < q.bias_length && !earlier; j0 += 32) {
-      const int64_t j = j0 + lane;
-      uint32_t same = __ballot_sync(0xffffffffu, j < q.bias_length && __ldg(ids + j) == token);
-      for (; same != 0; same &= same - 1) {
-        const int64_t k = j0 + __ffs(same) - 1;
-        earlier |= k < i;
-        bias += __ldg(values + k);
+  // of all its entries, in their order. (More entries than threads: each pass looks at those before and
+  // behind it in memory.)
+  for (int64_t from = 0; from < q.bias_length; from += kLogitsThreads) {
+    if (from > 0) fetch_bias(from);
+    bias_ids[threadIdx.x] = bias_id, bias_values[threadIdx.x] = bias_value;
+    __syncthreads();   // and the listed tokens are stored
+    if (bias_id >= first && bias_id >= 0 && bias_id < first + a.stretch) {
+      const int32_t* ids = q.bias_ids + row * q.bias_length;
+      const float* values = q.bias_values + row * q.bias_length;
+      const int here = static_cast<int>(q.bias_length - from < kLogitsThreads ? q.bias_length - from : kLogitsThreads);
+      bool earlier = false;
+      for (int64_t j = 0; j < from && !earlier; ++j) earlier = __ldg(ids + j) == bias_id;
+      for (int j = 0; j < static_cast<int>(threadIdx.x); ++j) earlier |= bias_ids[j] == bias_id;
+      if (!earlier) {
+        float bias = 0.f;
+        for (int j = threadIdx.x; j < here; ++j) bias += bias_ids[j] == bias_id ? bias_values[j] : 0.f;
+        for (int64_t j = from + here; j < q.bias_length; ++j) bias += __ldg(ids + j) == bias_id ? __ldg(values + j) : 0.f;
+        y[bias_id] = finish(bias_id, penalised(bias_logit, counts[static_cast<int>(bias_id - first)], kSeen, p) + bias);
       }
     }
-    if (!earlier && lane == 0) y[token] = finish(token, penalised(to_float(x[token]), counts[static_cast<int>(at)], kSeen, p) + bias);
+    __syncthreads();
   }
 }
 

@@ -518,6 +518,13 @@ def test_process_logits_counts_long_repetitions():
     assert float(out[0, 5]) == -100000.0 and int((out != 0).sum()) == 1
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bias", [255, 257, 700])
+def test_process_logits_long_bias_lists(dtype, bias):
+    inputs = logits_inputs(31, 2, 3000, 30, 40000 if bias == 700 else 60, bias, dtype)   # many entries of few tokens; counters of both widths
+    check_logits(K.process_logits(**inputs), inputs)
+
+
 def test_process_logits_refusals():
     inputs = logits_inputs(21, 3, 100, 5, 5, 2, torch.float32)
     for change, match in ((dict(prompt_tokens=inputs["prompt_tokens"].long()), "int32"), (dict(output_tokens=inputs["output_tokens"][:2]), "one row per row"),
