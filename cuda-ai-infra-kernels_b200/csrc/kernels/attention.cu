@@ -83,7 +83,7 @@ struct RowJoin {
 static_assert(kJoinWarps == 4, "columns of a row over the warps of a CTA");
 
 // Prompt calls: block (c, y) handles rows 8 y .. 8 y + 7 of the unit that CTA c left open.
-__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_cuts_kernel(const AttentionArgs a) {
+__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_cuts_kernel(const __grid_constant__ AttentionArgs a) {
   grid_launch_dependents();
   grid_dependency_wait();
   const CutRecord cut = a.cuts[blockIdx.x];
@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_cuts_kernel(co
 
 // Shared-prefix calls: block (x, h) handles rows 8 x .. 8 x + 7 of key head h: their part over the
 // prefix, and the one over their request's own keys.
-__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_rows_kernel(const AttentionArgs a) {
+__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_rows_kernel(const __grid_constant__ AttentionArgs a) {
   grid_launch_dependents();
   grid_dependency_wait();
   const int flat = blockIdx.x * 8 + (threadIdx.x & 7), head = blockIdx.y;
@@ -109,9 +109,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_rows_kernel(co
     join.unit(prefix_slot(a, unit, head), a.unit_rows, flat - unit * a.unit_rows, cut.first, cut.last);
   }
   if (sequence_of(a, 1 + request).m > 0) {
-    const int unit = g / a.unit_rows;
-    const CutRecord cut = a.cuts[own_record(a, request, head, unit)];
-    join.unit(own_slot(a, request, head, unit), own_pitch(a, unit), g - unit * a.unit_rows, cut.first, cut.last);
+    const CutRecord cut = a.cuts[own_record(a, request, head)];
+    join.unit(own_slot(a, request, head), a.group, g, cut.first, cut.last);
   }
   join.store(static_cast<int64_t>(request) * a.heads + head * a.group + g);
 }
@@ -219,7 +218,7 @@ Plan plan(AttentionArgs* a) {
   int64_t ranges;      // more CTAs than this would have nothing to do
   if (a->kind == kShared) {
     if (a->kv_heads > 65535) return {B200_ERR_INVALID_PROBLEM, false};   // a dimension of the join's grid
-    const int64_t prefix = units(static_cast<int64_t>(a->q_rows) * a->group), own = units(a->group) * a->q_rows;
+    const int64_t prefix = units(static_cast<int64_t>(a->q_rows) * a->group), own = a->q_rows;
     ranges = (prefix * longest + own * blocks(a->room)) * a->kv_heads;
     most = ranges * a->pair_cost + (prefix + own) * a->kv_heads * a->unit_cost;
   } else {
@@ -246,7 +245,7 @@ Workspace workspace_of(const AttentionArgs& a) {
   } else {
     const size_t prefix = units(static_cast<size_t>(a.q_rows) * a.group) * a.kv_heads;
     rows += prefix * a.unit_rows + static_cast<size_t>(a.q_rows) * a.heads;
-    records = prefix + static_cast<size_t>(a.q_rows) * a.kv_heads * units(a.group);
+    records = prefix + static_cast<size_t>(a.q_rows) * a.kv_heads;
   }
   Workspace w{};
   w.cuts = round(rows * sizeof(float2));

@@ -45,7 +45,7 @@ struct AttentionArgs {
   float scale_log2;                  // scale * log2(e): exponentials are powers of two
   int causal;
   int unit_rows;
-  int tokens;                        // of a unit; 0 where a group is larger than a unit, and units cut tokens
+  int tokens;                        // of a unit: it holds whole ones
   int token_shift;                   // its logarithm where it is a power of two, else -1
   int unit_cost, pair_cost;          // on the line: of a unit, of a block for a unit of more than half the rows
   int ctas;                          // ranges
@@ -112,13 +112,12 @@ __device__ __forceinline__ int visible_keys(const AttentionArgs& a, const Sequen
 }
 
 __device__ __forceinline__ int unit_count(const AttentionArgs& a, const Sequence& s) {
-  return a.tokens > 0 ? (s.n + a.tokens - 1) / a.tokens : (s.n * a.group + a.unit_rows - 1) / a.unit_rows;
+  return (s.n + a.tokens - 1) / a.tokens;
 }
 
 template <int kKeys>
 __device__ __forceinline__ int unit_blocks(const AttentionArgs& a, const Sequence& s, int unit) {
-  const int last = a.tokens > 0 ? (unit + 1) * a.tokens - 1 : ((unit + 1) * a.unit_rows - 1) / a.group;
-  return (visible_keys(a, s, min(last, s.n - 1)) + kKeys - 1) / kKeys;
+  return (visible_keys(a, s, min((unit + 1) * a.tokens, s.n) - 1) + kKeys - 1) / kKeys;
 }
 
 __device__ __forceinline__ int block_cost(const AttentionArgs& a, const Sequence& s, int unit) {
@@ -160,11 +159,6 @@ __device__ __noinline__ int length_before(const AttentionArgs& a, const Sequence
   const int regular = units < all ? units : all - 1;   // all but the last have all their rows
   const int rest = units == all ? unit_length<kKeys>(a, s, all - 1) : 0;
   if (a.kind == kShared || a.causal == 0) return (regular > 0 ? regular * unit_length<kKeys>(a, s, 0) : 0) + rest;
-  if (a.tokens == 0) {
-    int sum = rest;
-    for (int t = 0; t < regular; ++t) sum += unit_length<kKeys>(a, s, t);
-    return sum;
-  }
   // Unit t holds whole tokens; but for the last of all, its last token sees c + tokens * (t + 1) keys.
   const int tokens = a.tokens, c = s.m - s.n;
   const int blind = c >= 0 ? 0 : min(-c / tokens, regular);   // units that see nothing
@@ -348,15 +342,12 @@ __device__ __forceinline__ int prefix_units(const AttentionArgs& a) { return (a.
 __device__ __forceinline__ int64_t prefix_slot(const AttentionArgs& a, int unit, int head) {
   return (a.ctas + static_cast<int64_t>(unit) * a.kv_heads + head) * a.unit_rows;
 }
-__device__ __forceinline__ int64_t own_slot(const AttentionArgs& a, int request, int head, int unit) {
-  return (a.ctas + static_cast<int64_t>(prefix_units(a)) * a.kv_heads) * a.unit_rows +
-         (static_cast<int64_t>(request) * a.kv_heads + head) * a.group + unit * a.unit_rows;
+__device__ __forceinline__ int64_t own_slot(const AttentionArgs& a, int request, int head) {
+  return (a.ctas + static_cast<int64_t>(prefix_units(a)) * a.kv_heads) * a.unit_rows + (static_cast<int64_t>(request) * a.kv_heads + head) * a.group;
 }
-__device__ __forceinline__ int own_pitch(const AttentionArgs& a, int unit) { return min(a.unit_rows, a.group - unit * a.unit_rows); }
 __device__ __forceinline__ int64_t prefix_record(const AttentionArgs& a, int unit, int head) { return static_cast<int64_t>(unit) * a.kv_heads + head; }
-__device__ __forceinline__ int64_t own_record(const AttentionArgs& a, int request, int head, int unit) {
-  const int units = (a.group + a.unit_rows - 1) / a.unit_rows;
-  return (static_cast<int64_t>(prefix_units(a)) + static_cast<int64_t>(request) * units + unit) * a.kv_heads + head;
+__device__ __forceinline__ int64_t own_record(const AttentionArgs& a, int request, int head) {
+  return (static_cast<int64_t>(prefix_units(a)) + request) * a.kv_heads + head;
 }
 
 __device__ __forceinline__ bool is_partial(const AttentionArgs& a, const Segment& g) { return a.kind == kShared || !g.whole; }
@@ -367,8 +358,8 @@ __device__ __forceinline__ int64_t slot_of(const AttentionArgs& a, const Segment
   if (!g.opens) return continued_slot(a, blockIdx.x);
   if (a.kind == kPrompt) return continued_slot(a, a.ctas + blockIdx.x);
   if (g.seq.source == 0) return prefix_slot(a, g.unit, g.head);
-  *pitch = own_pitch(a, g.unit);
-  return own_slot(a, g.seq.batch, g.head, g.unit);
+  *pitch = a.group;
+  return own_slot(a, g.seq.batch, g.head);
 }
 
 // The record of an opened unit. To be called by one thread of the CTA for each segment, and, in a
@@ -380,7 +371,7 @@ __device__ __forceinline__ void record(const AttentionArgs& a, const Segment& g)
   if (!g.opens || !is_partial(a, g)) return;
   const CutRecord r{g.first_cta, g.last_cta, min(a.unit_rows, g.seq.n * a.group - g.unit * a.unit_rows), g.seq.q_row, g.head, g.unit * a.unit_rows};
   if (a.kind == kPrompt) a.cuts[blockIdx.x] = r;
-  else a.cuts[g.seq.source == 0 ? prefix_record(a, g.unit, g.head) : own_record(a, g.seq.batch, g.head, g.unit)] = r;
+  else a.cuts[g.seq.source == 0 ? prefix_record(a, g.unit, g.head) : own_record(a, g.seq.batch, g.head)] = r;
 }
 
 // Output row of row `flat` of a sequence's rows of a key head.
