@@ -144,7 +144,7 @@ size_t element_bytes(int dtype) { return dtype == B200_FP32 ? 4 : 2; }
 int check_common(int dtype, int heads, int kv_heads, int dim, float scale) {
   if (dtype < B200_FP32 || dtype > B200_BF16) return B200_ERR_INVALID_ARGUMENT;
   if (heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || dim <= 0) return B200_ERR_INVALID_ARGUMENT;
-  if (!(scale > 0.f) || scale > 3.0e38f) return B200_ERR_INVALID_ARGUMENT;
+  if (!(scale > 0.f) || scale > 2.0e38f) return B200_ERR_INVALID_ARGUMENT;
   if (dim % 8 != 0 || dim > 128 || heads / kv_heads > 128) return B200_ERR_NOT_SUPPORTED;
   return B200_OK;
 }

@@ -206,7 +206,7 @@ struct WorkStart {
 };
 
 struct WorkScratch {
-  int sums[32];
+  int64_t sums[32];
   WorkStart start;
 };
 
@@ -217,31 +217,34 @@ __device__ __forceinline__ WorkStart find_range(const AttentionArgs& a, WorkScra
   const int chunk = (count + kThreads - 1) / kThreads;
   const int lo = min(static_cast<int>(threadIdx.x) * chunk, count), hi = min(lo + chunk, count);
   Sequence seq{};
-  int mine = 0, size = 0;
+  int size = 0;
+  int64_t mine = 0;   // offsets that overlap could make the line longer than the launcher counted on
   for (int s = lo; s < hi; ++s) {
     seq = sequence_of(a, s);
     const int units = unit_count(a, seq);
     size = a.kv_heads * length_before<kKeys>(a, seq, units, units);
     mine += size;
   }
-  int upto = mine;   // inclusive over the warp
+  int64_t upto = mine;   // inclusive over the warp
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int other = __shfl_up_sync(0xffffffffu, upto, o);
+    const int64_t other = __shfl_up_sync(0xffffffffu, upto, o);
     if ((threadIdx.x & 31) >= o) upto += other;
   }
   if ((threadIdx.x & 31) == 31) scratch->sums[threadIdx.x >> 5] = upto;
   WorkStart& start = scratch->start;
   if (threadIdx.x == 0) start.sequence = -1;
   __syncthreads();
-  int before = upto - mine, total = 0;
+  int64_t ahead = upto - mine, whole = 0;
   for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < static_cast<int>(threadIdx.x >> 5)) before += scratch->sums[w];
-    total += scratch->sums[w];
+    if (w < static_cast<int>(threadIdx.x >> 5)) ahead += scratch->sums[w];
+    whole += scratch->sums[w];
   }
+  const int total = whole <= 0x7fffffff ? static_cast<int>(whole) : 0;   // too long: nothing is done
+  int before = static_cast<int>(min(ahead, static_cast<int64_t>(total)));
   const Ranges ranges(total, a.ctas);
   const int begin = ranges.begin(blockIdx.x), length = ranges.begin(blockIdx.x + 1) - begin;
-  if (length > 0 && begin >= before && begin < before + mine) {
+  if (length > 0 && begin >= before && begin < ahead + mine) {
     int s = lo;
     if (hi - lo > 1) {
       for (; s < hi; ++s) {

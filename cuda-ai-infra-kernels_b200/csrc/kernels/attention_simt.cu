@@ -8,6 +8,9 @@
 // shared-memory pipe has to keep up: with 8 rows a thread loads 12 granules per 128 multiply-adds.
 // Both products run on packed pairs (two multiply-adds per instruction): S over even and odd d apart.
 //
+// 2048 and 1000 causal tokens, 16 heads of 64: 354 us, 29 TFLOP/s of the 70 that the pipe reaches on
+// multiply-adds alone (64-row tiles, two CTAs per SM: 453; one buffer filled between barriers: 466).
+//
 // Keys and values have one buffer each. The next keys are copied (cp.async) while the exponentials and
 // the second product run, the next values while the first product does.
 #include "attention.cuh"
@@ -56,7 +59,7 @@ __device__ __forceinline__ void copy_rows(float* dst, const float* src, int64_t 
 __device__ __forceinline__ ulonglong2 pairs_at(const float* p) { return *reinterpret_cast<const ulonglong2*>(p); }
 
 template <int kRows, int kThreads, int kColumns>
-__global__ void __launch_bounds__(kThreads) attention_simt_kernel(const __grid_constant__ AttentionArgs a) {
+__global__ void __launch_bounds__(kThreads, kRows == 16 ? 4 : kRows == 64 ? 2 : 1) attention_simt_kernel(const __grid_constant__ AttentionArgs a) {
   constexpr int kPer = kRows / (kThreads / 16);   // rows of a thread
   constexpr int kQuads = kColumns / 64;           // groups of four of its columns of O
   constexpr int kPitchP = kKeys + 4;
@@ -113,7 +116,7 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(const __grid_c
       copy_wait<1>();    // the keys
       __syncthreads();
       uint64_t x2[kPer][4] = {};   // sums over even and odd d
-#pragma unroll 2
+#pragma unroll 4
       for (int d = 0; d < a.dim; d += 4) {
         ulonglong2 qv[kPer], kv[4];
 #pragma unroll
@@ -154,7 +157,7 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(const __grid_c
       }
       copy_wait<1>();    // the values
       __syncthreads();
-#pragma unroll 2
+#pragma unroll 4
       for (int key = 0; key < kKeys; key += 4) {
         float4 p[kPer];
 #pragma unroll
@@ -237,9 +240,9 @@ void plan_attention_simt(AttentionArgs* a, int sms) {
   a->tokens = tile / a->group;
   a->unit_rows = a->tokens * a->group;
   a->unit_cost = 1, a->pair_cost = 1;
-  // As many CTAs as an SM's shared memory holds, up to what its registers allow.
+  // As many CTAs as an SM's shared memory holds, up to what its registers do.
   const int fit = static_cast<int>((227 * 1024) / (simt_smem_bytes(tile, a->dim) + 2048));
-  const int most = tile == 16 ? 5 : tile == 64 ? 2 : 1;
+  const int most = tile == 16 ? 4 : tile == 64 ? 2 : 1;
   a->ctas = sms * (fit < 1 ? 1 : fit < most ? fit : most);
 }
 

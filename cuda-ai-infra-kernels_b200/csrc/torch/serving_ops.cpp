@@ -63,7 +63,7 @@ b200_rows_view rows_view(const torch::Tensor& t, int64_t row_dim) {
 
 float scale_or_default(const c10::optional<double>& scale, int64_t dim) {
   const float s = static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(dim)));
-  TORCH_CHECK(s > 0.f && s <= 3.0e38f, "scale must be positive and finite");
+  TORCH_CHECK(s > 0.f && s <= 2.0e38f, "scale must be positive and finite");
   return s;
 }
 
