@@ -47,7 +47,7 @@ struct AttentionArgs {
   int unit_rows;
   int tokens;                        // of a unit: it holds whole ones
   int token_shift;                   // its logarithm where it is a power of two, else -1
-  int unit_cost, pair_cost;          // on the line: of a unit, of a block for a unit of more than half the rows
+  int unit_cost, pair_shift;         // on the line: of a unit; logarithm of a block's for a unit of more than half the rows
   int ctas;                          // ranges
   // Partial results, in slots of some rows: maximum (scaled, base 2) and denominator [row], and the sum,
   // not divided by it, as [dim / 4][row][4], so that the threads of a warp, which own one row
@@ -94,14 +94,16 @@ __device__ __forceinline__ Sequence sequence_of(const AttentionArgs& a, int s) {
     }
     return r;
   }
-  r.q_row = clamp_int(__ldg(a.cu_q + s), 0, a.q_rows);
+  const int next = min(s + 1, a.sequences);   // all four on their way at once
+  const int q0 = __ldg(a.cu_q + s), q1 = __ldg(a.cu_q + next), k0 = __ldg(a.cu_k + s), k1 = __ldg(a.cu_k + next);
+  r.q_row = clamp_int(q0, 0, a.q_rows);
+  r.k_row = clamp_int(k0, 0, a.k_rows);
   if (s == a.sequences) {
     r.n = a.q_rows - r.q_row;
-    return r;
+  } else {
+    r.n = clamp_int(q1, r.q_row, a.q_rows) - r.q_row;
+    r.m = clamp_int(k1, r.k_row, a.k_rows) - r.k_row;
   }
-  r.n = clamp_int(__ldg(a.cu_q + s + 1), r.q_row, a.q_rows) - r.q_row;
-  r.k_row = clamp_int(__ldg(a.cu_k + s), 0, a.k_rows);
-  r.m = clamp_int(__ldg(a.cu_k + s + 1), r.k_row, a.k_rows) - r.k_row;
   return r;
 }
 
@@ -120,8 +122,8 @@ __device__ __forceinline__ int unit_blocks(const AttentionArgs& a, const Sequenc
   return (visible_keys(a, s, min((unit + 1) * a.tokens, s.n) - 1) + kKeys - 1) / kKeys;
 }
 
-__device__ __forceinline__ int block_cost(const AttentionArgs& a, const Sequence& s, int unit) {
-  return s.n - unit * a.tokens > a.tokens / 2 ? a.pair_cost : 1;
+__device__ __forceinline__ int block_shift(const AttentionArgs& a, const Sequence& s, int unit) {   // logarithm of its length
+  return s.n - unit * a.tokens > a.tokens / 2 ? a.pair_shift : 0;
 }
 
 // Length of a unit on the line. A prompt's unit that sees no key is there all the same: somebody has
@@ -129,7 +131,7 @@ __device__ __forceinline__ int block_cost(const AttentionArgs& a, const Sequence
 template <int kKeys>
 __device__ __forceinline__ int unit_length(const AttentionArgs& a, const Sequence& s, int unit) {
   const int blocks = unit_blocks<kKeys>(a, s, unit);
-  return blocks > 0 || a.kind == kPrompt ? blocks * block_cost(a, s, unit) + a.unit_cost : 0;
+  return blocks > 0 || a.kind == kPrompt ? (blocks << block_shift(a, s, unit)) + a.unit_cost : 0;
 }
 
 // sum over i = 0 .. n - 1 of floor((a i + b) / m), for a, b >= 0: the whole multiples of m in a and b
@@ -181,7 +183,7 @@ __device__ __noinline__ int length_before(const AttentionArgs& a, const Sequence
     };
     sum += static_cast<int>(below(first + n) - below(first));
   }
-  return sum * a.pair_cost + regular * a.unit_cost + rest;
+  return (sum << a.pair_shift) + regular * a.unit_cost + rest;
 }
 
 // ------------------------------------------------------------------------- finding a CTA's work
@@ -189,7 +191,8 @@ __device__ __noinline__ int length_before(const AttentionArgs& a, const Sequence
 // Ranges of the line: the first total % ctas are one longer than the rest.
 struct Ranges {
   int quotient, longer;
-  __device__ __forceinline__ Ranges(int total, int ctas) : quotient(total / ctas), longer(total - total / ctas * ctas) {}
+  __device__ __forceinline__ Ranges(int total, int ctas) : quotient(total / ctas), longer(total - quotient * ctas) {}
+  Ranges() = default;
   __device__ __forceinline__ int begin(int c) const { return c * quotient + min(c, longer); }
   __device__ __forceinline__ int holder(int position) const {
     const int boundary = longer * (quotient + 1);
@@ -202,7 +205,8 @@ struct WorkStart {
   Sequence seq;
   int units;                  // of a head of the sequence
   int head, unit, offset;     // offset: into the unit
-  int total, begin, length;   // of the line; the range
+  Ranges ranges;
+  int begin, length;          // of this range
 };
 
 struct WorkScratch {
@@ -256,7 +260,7 @@ __device__ __forceinline__ WorkStart find_range(const AttentionArgs& a, WorkScra
       }
     }
     const int per_head = size / a.kv_heads, head = (begin - before) / per_head;
-    start = WorkStart{s, seq, unit_count(a, seq), head, 0, begin - before - head * per_head, total, begin, length};
+    start = WorkStart{s, seq, unit_count(a, seq), head, 0, begin - before - head * per_head, ranges, begin, length};
   }
   __syncthreads();
   WorkStart found = start;
@@ -297,17 +301,17 @@ struct SegmentWalk {
   Sequence seq;
   int head, unit, offset;
 
-  __device__ __forceinline__ SegmentWalk(const AttentionArgs& args, const WorkStart& start) : a(args), ranges(start.total, args.ctas) {
+  __device__ __forceinline__ SegmentWalk(const AttentionArgs& args, const WorkStart& start) : a(args), ranges(start.ranges) {
     position = start.begin, end = start.sequence < 0 ? start.begin : start.begin + start.length;
     sequence = start.sequence, seq = start.seq, units = start.units, head = start.head, unit = start.unit, offset = start.offset;
   }
 
   __device__ __forceinline__ bool next(Segment* out) {
     while (position < end) {
-      const int blocks = unit_blocks<kKeys>(a, seq, unit), length = unit_length<kKeys>(a, seq, unit), cost = block_cost(a, seq, unit);
+      const int blocks = unit_blocks<kKeys>(a, seq, unit), length = unit_length<kKeys>(a, seq, unit), shift = block_shift(a, seq, unit);
       const int from = offset, to = min(length, offset + end - position);
       const int unit_position = position - from;
-      Segment g{seq, head, unit, max(from - a.unit_cost, 0) / cost, max(to - a.unit_cost, 0) / cost, false, false, 0, 0};
+      Segment g{seq, head, unit, max(from - a.unit_cost, 0) >> shift, max(to - a.unit_cost, 0) >> shift, false, false, 0, 0};
       position += to - from;
       offset = to;
       if (to == length) {   // on to the next unit
@@ -328,7 +332,8 @@ struct SegmentWalk {
       // a unit leaves an empty partial result: the join counts on one from every CTA on the way.
       if (blocks > 0 ? g.block_end > 0 : length > 0 && to == length) {
         g.opens = g.block_begin == 0, g.whole = g.opens && g.block_end == blocks;   // block_end > 0 or no blocks at all
-        g.first_cta = blockIdx.x, g.last_cta = g.whole ? blockIdx.x : ranges.holder(unit_position + length - 1);
+        g.first_cta = g.last_cta = blockIdx.x;
+        if (g.opens && !g.whole) g.last_cta = ranges.holder(unit_position + length - 1);
         *out = g;
         return true;
       }

@@ -239,7 +239,7 @@ void plan_attention_simt(AttentionArgs* a, int sms) {
   const int tile = tile_of(*a);
   a->tokens = tile / a->group;
   a->unit_rows = a->tokens * a->group;
-  a->unit_cost = 1, a->pair_cost = 1;
+  a->unit_cost = 1, a->pair_shift = 0;
   // As many CTAs as an SM's shared memory holds, up to what its registers do.
   const int fit = static_cast<int>((227 * 1024) / (simt_smem_bytes(tile, a->dim) + 2048));
   const int most = tile == 16 ? 4 : tile == 64 ? 2 : 1;

@@ -688,7 +688,7 @@ void plan_attention_umma(AttentionArgs* a, int sms) {
   // Tiles hold whole tokens: a copy brings (dim, group, tokens) boxes.
   a->tokens = 2 * (kTile / a->group);
   a->unit_rows = a->tokens * a->group;
-  a->unit_cost = 3, a->pair_cost = 2;   // a block of one tile takes about 1.2 us, a unit beside its blocks 2 to 3
+  a->unit_cost = 3, a->pair_shift = 1;   // a block of one tile takes about 1.2 us, a unit beside its blocks 2 to 3
   a->ctas = sms;
 }
 
