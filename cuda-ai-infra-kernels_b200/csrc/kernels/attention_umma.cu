@@ -3,8 +3,8 @@
 // For a tile of 128 rows and 64 keys: S = Q K^T into tensor memory (tcgen05.mma, both operands in
 // shared memory), the row maxima and P = 2^(scale S - m) in registers, one thread per row, P back into
 // tensor memory as a 16-bit operand in columns that held S, and O += P V with P read from there. O
-// stays in tensor memory for the whole unit. P is rounded to the operand type (relative 2^-9 or 2^-12
-// per probability, of the size of the output's own rounding); the denominator adds up the unrounded
+// stays in tensor memory for the whole unit. P is rounded to the operand type (at most 2^-8 or 2^-11
+// of a probability, as the output's own rounding); the denominator adds up the unrounded
 // FP32 values.
 //
 // Two streams, each with its own group of four warps, O and S: the two row tiles of a unit of 256
@@ -37,7 +37,7 @@ cudaError_t attention_status_read_clear(uint32_t* word) { return status_word_rea
 namespace {
 
 constexpr int kThreads = 384;
-// Registers: 168 per thread at launch; a softmax thread holds a row of 128 scores and takes more.
+// Registers: 168 per thread at launch; a softmax thread holds 64 scores, or 32 columns of both accumulators.
 constexpr int kSoftmaxRegisters = 216, kOtherRegisters = 72;
 static_assert(256 * kSoftmaxRegisters + 128 * kOtherRegisters <= kThreads * 168, "registers of the CTA");
 constexpr int kTile = 128;          // rows of a tile, keys of a block
@@ -514,7 +514,7 @@ __device__ __forceinline__ void softmax_role(const UmmaAttentionArgs& p, Shared*
     }
     if (items > 1) drain_phase ^= 1;
     // Rows of one tile that two streams worked on: the same thread of both warp groups owns them, and
-    // each finishes every other 32 columns.
+    // each finishes 64 of their columns.
     const bool joined = !pair && halves > 1;
     float mine = 1.f, other = 0.f, total = row.l, base = row.m;
     if (joined) {

@@ -127,9 +127,12 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_kernel(const LogitsArgs
   for (int i = threadIdx.x; i < a.stretch / (kNarrow ? 8 : 4); i += kLogitsThreads) reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
   grid_dependency_wait();
-  const int64_t row = blockIdx.x / a.stretches;
+  // The first stretches of all rows come first: frequent tokens have low numbers as a rule, and their
+  // counting takes longest.
+  const unsigned rows = static_cast<unsigned>(q.rows), stretch = blockIdx.x / rows;
+  const int64_t row = blockIdx.x - stretch * rows;
   const int64_t lead = (row * q.vocab) % kVec;
-  const int64_t first = static_cast<int64_t>(blockIdx.x % a.stretches) * a.stretch - lead;   // token of position 0; may be negative
+  const int64_t first = static_cast<int64_t>(stretch) * a.stretch - lead;   // token of position 0; may be negative
   if (first >= q.vocab) return;
   RowPenalties p{1.f, 0.f, 0.f};
   if (q.repetition != nullptr) p.repetition = q.repetition[row];
