@@ -269,7 +269,9 @@ struct MmaIssuer {
     v_desc = umma_smem_desc(smem_u32(smem) + 2 * S::kTileBytes, S::kHalfBytes, 1024, kUmmaSwizzle128B);
   }
   __device__ __forceinline__ bool arrived(uint32_t at) const { return mbar_wait(&b->full[at % S::kSlots], at / S::kSlots & 1, kSiteAttention); }
-  __device__ __forceinline__ void release(uint32_t at) const { umma_commit(&b->empty[at % S::kSlots]); }   // both streams count for a block
+
+  // Hands a block of the ring back when the products so far are done. Of a single tile only; see softmax_role.
+  __device__ __forceinline__ void release(uint32_t at) const { umma_commit(&b->empty[at % S::kSlots]); }
 
   // Item j is S buffer j & 1, over 64 keys of a block: both halves of it in turn, or (one tile) the
   // stream's own.
@@ -291,7 +293,7 @@ struct MmaIssuer {
       umma_f16(at, umma_desc_advance(qd, offset), umma_desc_advance(kd, offset), kIdescS, step > 0);
     }
     umma_commit(&b->s_full[s][j & 1]);
-    if (!kPair || (j & 1) == 1 || j + 1 == items) release(load_of<kPair>(j));
+    if (!kPair) release(load_of<kPair>(j));
     if (j + 1 == items) umma_commit(&b->q_empty);
   }
   template <bool kPair>
@@ -326,7 +328,6 @@ struct MmaIssuer {
       }
       if (j + 2 == items) umma_commit(&b->drained[s]);
       if (j + 1 == items) umma_commit(&b->o_full[s]);
-      if (kPair && ((j & 1) == 1 || j + 1 == items)) release(at + 1);
     }
     ++own_segment;
     return true;
@@ -442,7 +443,7 @@ __device__ __forceinline__ void stage_columns(uint8_t* stage, int lane, int half
                                                   pack<kBf16>(y[8 * i + 4], y[8 * i + 5]), pack<kBf16>(y[8 * i + 6], y[8 * i + 7]));
 }
 
-template <bool kBf16>
+template <bool kBf16, uint32_t kSlots>
 __device__ __forceinline__ void softmax_role(const UmmaAttentionArgs& p, Shared* b, uint8_t* staging, uint32_t tmem) {
   const AttentionArgs& a = p.a;
   const int s = threadIdx.x >> 7;                    // stream
@@ -457,7 +458,7 @@ __device__ __forceinline__ void softmax_role(const UmmaAttentionArgs& p, Shared*
   const int chunks = (a.dim + 31) / 32;
   EntryReader reader{b};
   bool ok = true;
-  uint32_t s_phase = 0, drain_phase = 0, o_count[2] = {0, 0}, met = 0;
+  uint32_t load = 0, s_phase = 0, drain_phase = 0, o_count[2] = {0, 0}, met = 0;
   // All eight warps; a bounded wait, which a plain barrier has not.
   const auto meet = [&]() {
     __syncwarp();
@@ -489,11 +490,20 @@ __device__ __forceinline__ void softmax_role(const UmmaAttentionArgs& p, Shared*
     const int seen = live ? clamp_int(ahead + token0 + token_r, 0, keys) : 0;
     // All rows of the warp that are there see at least what its first row sees.
     const int seen_by_all = clamp_int(ahead + token0 + token_warp, 0, keys);
+    // Two tiles hand blocks of the ring back here, one arrival per stream: scores that have arrived tell
+    // that their keys have been read, and the values of the half before the last one too. Commits by the
+    // MMA threads would say so earlier, but cost those threads, which everybody waits for, 130 cycles
+    // each (16384 tokens 1073 -> 996 us). A single tile passes through the ring twice as fast, and needs
+    // the places back at once (64 requests 142 us this way, 120 by commits).
+    const auto hand_back = [&](int j, int values) {   // keys or values of item j, if it is its block's last
+      if (pair && r == 0 && j >= 0 && ((j & 1) == 1 || j + 1 == items)) mbar_arrive(&b->empty[(load + 2 * (j >> 1) + values) % kSlots]);
+    };
     for (int j = 0; j < items; ++j) {
       const uint32_t half = j & 1;
       const int key0 = (pair ? j : 2 * j + s) * kHalf;
       ok = __all_sync(0xffffffffu, ok && mbar_wait(&b->s_full[s][half], s_phase >> half & 1, kSiteAttention));
       s_phase ^= 1u << half;
+      hand_back(j, 0), hand_back(j - 2, 1);
       if (ok && warp_live) {
         tcgen05_fence_after_sync();
         // Scores of the half after are issued behind the products of the half before; the last half
@@ -513,6 +523,12 @@ __device__ __forceinline__ void softmax_role(const UmmaAttentionArgs& p, Shared*
       if (lane == 0) mbar_arrive(&b->p_ready[s][half]);
     }
     if (items > 1) drain_phase ^= 1;
+    if (items > 0) {
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(&b->o_full[s], o_count[s] & 1, kSiteAttention));
+      ++o_count[s];
+      hand_back(items - 2, 1), hand_back(items - 1, 1);
+    }
+    load += 2 * blocks;
     // Rows of one tile that two streams worked on: the same thread of both warp groups owns them, and
     // each finishes 64 of their columns.
     const bool joined = !pair && halves > 1;
@@ -527,12 +543,11 @@ __device__ __forceinline__ void softmax_role(const UmmaAttentionArgs& p, Shared*
       total = row.l * mine + peer.y * other;
       meet();   // read by all before the next segment writes
     }
-#pragma unroll
-    for (int stream = 0; stream < 2; ++stream) {
-      if ((pair || stream == 0 || joined) && blocks > 0) {   // the stream has an accumulator
-        if (stream == s || joined) ok = __all_sync(0xffffffffu, ok && mbar_wait(&b->o_full[stream], o_count[stream] & 1, kSiteAttention));
-        ++o_count[stream];
-      }
+    if (pair || joined) {   // the other stream has an accumulator too
+      if (joined) ok = __all_sync(0xffffffffu, ok && mbar_wait(&b->o_full[s ^ 1], o_count[s ^ 1] & 1, kSiteAttention));
+      if (blocks > 0) ++o_count[s ^ 1];
+    } else if (s == 1 && blocks > 0) {
+      ++o_count[0];
     }
     tcgen05_fence_after_sync();
     if (ok && warp_live && (pair || s == 0 || joined)) {
@@ -639,7 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_umma_kernel(const __gri
   const WorkStart start = find_range<kUmmaKeyBlock, kThreads>(p.a, &b.scratch);
   if (warp < 8) {
     registers_raise<kSoftmaxRegisters>();
-    softmax_role<kBf16>(p, &b, smem + S::kStaging, tmem);
+    softmax_role<kBf16, S::kSlots>(p, &b, smem + S::kStaging, tmem);
   } else {
     registers_lower<kOtherRegisters>();
     if (warp == 8 && lane == 0) copy_role<kDim>(p, smem, &b);
