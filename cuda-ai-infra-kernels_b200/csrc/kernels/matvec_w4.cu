@@ -14,12 +14,16 @@
 // subtracting 1024 + zero or 128 + zero leaves c - zero, exact. Each step of K lies inside one group:
 // its FP32 product is multiplied by the group's scale when it is added to the running sum.
 //
-// What it measured: one BF16 row by 28672 x 8192 (117 MB of weights) 44.8 us, FP16 42.1, against 18.5 for
-// the weights at the copy bandwidth: issue slots 58 % busy, the integer pipe 61 %, HBM 30 %. Four
-// things that did not help, all timed side by side: 32 rows per warp (x shared, half the warps: 51.5);
-// more warps by fewer registers (51.6 with five CTAs per SM instead of four, 55.3 with six); the warps
-// side by side along K instead of in ranges (45.6); and integer matrix instructions on the raw codes with
-// x in signed 8-bit digits, a third of the instructions (62).
+// What it measured: one BF16 row by 28672 x 8192 (117 MB of weights) 36.8 us, FP16 35.0, against 18.5 for
+// the weights at the copy bandwidth: issue slots 52 % busy, the integer pipe 58 %. What brought it there
+// from 44.7: a code's mask and its base in one instruction (38.5), and the divisions that place a warp in
+// its row done by the host, the zero point of symmetric weights made once (36.8). What did not help, all
+// timed side by side: 32 rows per warp (x shared, half the warps: 51.5 against 44.8); more warps by fewer
+// registers (45.3 with five CTAs per SM instead of four); the warps side by side along K instead of in
+// ranges (45.6 against 44.8); the next step's weights loaded a step ahead (39.3); x laid out as pairs in
+// shared memory (37.3 against 38.5 here, but 21.0 against 18.3 for 11008 x 4096 in groups of 32 and 9.6
+// against 8.7 for four rows by 4096 x 4096); and integer matrix instructions on the raw codes with x in
+// signed 8-bit digits, a third of the instructions (62 against 44.8).
 //
 // FP32 x is written as the sum of three BF16 numbers (8 + 8 + 8 bits, by truncation: exact), which take
 // three columns of the instruction and are added up at the end, so that products and sums are as
@@ -40,6 +44,7 @@ constexpr int kMaxRows = 16;
 
 struct W4Args {
   b200_matvec_w4_problem q;
+  int groups, steps, group_steps;   // groups of a row, steps of a row and of a group
 };
 
 template <typename T> struct Pair;
@@ -82,21 +87,28 @@ __device__ __forceinline__ ZeroPair zero_pair(uint32_t z) {
   // 1024 + z as it is; a code in bits 4..7 reads 1024 + 16 c and is divided by 16, which leaves 64 + c.
   return {Pair<T>::kBase | twice, 0xd400d400u | twice << 4};   // FP16: -(64 + z)
 }
+// (v & kMask) | base in one instruction.
+template <uint32_t kMask>
+__device__ __forceinline__ uint32_t masked_onto(uint32_t base, uint32_t v) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(v), "n"(kMask), "r"(base));
+  return r;
+}
 template <typename T>
-__device__ __forceinline__ void decode(uint32_t (&out)[4], uint32_t w, const ZeroPair& zero) {
+__device__ __forceinline__ void decode(uint32_t (&out)[4], uint32_t w, const ZeroPair& zero, uint32_t base) {
   if constexpr (std::is_same<T, __half>::value) {
     const uint32_t upper = w >> 8;
     const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00));
     const auto high = [&](uint32_t v) {
-      const uint32_t c = (v & 0x00f000f0u) | Pair<T>::kBase;
+      const uint32_t c = masked_onto<0x00f000f0u>(base, v);
       const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&c), sixteenth, *reinterpret_cast<const __half2*>(&zero.high));
       return *reinterpret_cast<const uint32_t*>(&r);
     };
-    out[0] = Pair<T>::sub((w & 0x000f000fu) | Pair<T>::kBase, zero.low), out[1] = high(w);
-    out[2] = Pair<T>::sub((upper & 0x000f000fu) | Pair<T>::kBase, zero.low), out[3] = high(upper);
+    out[0] = Pair<T>::sub(masked_onto<0x000f000fu>(base, w), zero.low), out[1] = high(w);
+    out[2] = Pair<T>::sub(masked_onto<0x000f000fu>(base, upper), zero.low), out[3] = high(upper);
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) out[j] = Pair<T>::sub((w >> (4 * j) & 0x000f000fu) | Pair<T>::kBase, zero.low);
+    for (int j = 0; j < 4; ++j) out[j] = Pair<T>::sub(masked_onto<0x000f000fu>(base, w >> (4 * j)), zero.low);
   }
 }
 
@@ -168,13 +180,13 @@ __global__ void __launch_bounds__(kWarps * 32) matvec_w4_kernel(const W4Args a) 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quad = lane >> 2, t = lane & 3;
   const int row0 = blockIdx.x * 16;
-  const int groups = q.k / q.group, group_steps = q.group / kStep;
-  const int steps = q.k / kStep;
+  const int groups = a.groups, group_steps = a.group_steps, steps = a.steps;
   const int begin = static_cast<int>(static_cast<int64_t>(steps) * warp / kWarps), end = static_cast<int>(static_cast<int64_t>(steps) * (warp + 1) / kWarps);
   // This thread's two weight rows. Rows behind the last are read as the last one and not stored.
   const uint8_t* w[2];
   int64_t at[2];   // of the group's scale and zero
-  int group = begin / group_steps, left = (group + 1) * group_steps - begin;   // steps left in the group
+  const int group = group_steps == 1 ? begin : begin / group_steps;
+  int left = (group + 1) * group_steps - begin;   // steps left in the group
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int64_t r = min(row0 + 8 * i + quad, q.n - 1);
@@ -185,6 +197,9 @@ __global__ void __launch_bounds__(kWarps * 32) matvec_w4_kernel(const W4Args a) 
   float total[kTiles][4] = {};
   float scale[2];
   ZeroPair zero[2];
+  uint32_t base;   // a register that the compiler takes for no constant, which would cost an instruction per use
+  asm volatile("mov.b32 %0, %1;" : "=r"(base) : "n"(Pair<T>::kBase));
+  zero[0] = zero[1] = zero_pair<T>(8);
   bool fresh = true;
 #pragma unroll 2
   for (int s = begin; s < end; ++s) {
@@ -195,7 +210,7 @@ __global__ void __launch_bounds__(kWarps * 32) matvec_w4_kernel(const W4Args a) 
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         scale[i] = scale_at(q.scales, q.scale_dtype, at[i]);
-        zero[i] = zero_pair<T>(q.zeros == nullptr ? 8u : __ldg(q.zeros + at[i]) & 15u);
+        if (q.zeros != nullptr) zero[i] = zero_pair<T>(__ldg(q.zeros + at[i]) & 15u);
         ++at[i];
       }
     }
@@ -206,7 +221,7 @@ __global__ void __launch_bounds__(kWarps * 32) matvec_w4_kernel(const W4Args a) 
     for (int i = 0; i < kBytes / 4; ++i) {
       uint32_t m[2][4];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) decode<T>(m[r], p[r].w[i], zero[r]);
+      for (int r = 0; r < 2; ++r) decode<T>(m[r], p[r].w[i], zero[r], base);
       const uint32_t first[4] = {m[0][0], m[1][0], m[0][1], m[1][1]}, second[4] = {m[0][2], m[1][2], m[0][3], m[1][3]};
       const int64_t k = static_cast<int64_t>(s) * kStep + t * 2 * kBytes + i * 8;
 #pragma unroll
@@ -250,7 +265,7 @@ int launch(const b200_matvec_w4_problem& q, cudaStream_t s) {
   const GemmLaunchAttributes attrs = gemm_launch_attributes(1);
   cfg.attrs = const_cast<cudaLaunchAttribute*>(attrs.list);
   cfg.numAttrs = attrs.count;
-  if (cudaLaunchKernelEx(&cfg, matvec_w4_kernel<T, kTiles, kBytes>, W4Args{q}) != cudaSuccess) return launch_failed();
+  if (cudaLaunchKernelEx(&cfg, matvec_w4_kernel<T, kTiles, kBytes>, W4Args{q, q.k / q.group, q.k / (8 * kBytes), q.group / (8 * kBytes)}) != cudaSuccess) return launch_failed();
   return launch_status();
 }
 
