@@ -6,7 +6,7 @@
 // 5th-generation tensor cores would want 128 weight rows per tile in shared memory, a detour for
 // bytes that are used once; here they go from global memory to registers to the multiply.
 //
-// A warp owns 16 rows of weights and a range of K. The sum over k does not care about its order, so
+// A warp owns 16 or 32 rows of weights and a range of K. The sum over k does not care about its order, so
 // each of the four threads that share a row takes its own run of consecutive weights (kBytes bytes
 // per load) instead of the interleaved pairs that the instruction nominally wants, and loads the
 // same run of x. Nibbles i and i + 4 of a 32-bit word become one pair of 16-bit values: the bits of
@@ -15,7 +15,7 @@
 // its FP32 product is multiplied by the group's scale when it is added to the running sum.
 //
 // What it measured: one BF16 row by 28672 x 8192 (117 MB of weights) 36.8 us, FP16 35.0, against 18.5 for
-// the weights at the copy bandwidth: issue slots 52 % busy, the integer pipe 58 %. What brought it there
+// the weights at the copy bandwidth: issue slots 52 % busy, the integer pipe 58 %; 16 rows 71. What brought it there
 // from 44.7: a code's mask and its base in one instruction (38.5), and the divisions that place a warp in
 // its row done by the host, the zero point of symmetric weights made once (36.8). What did not help, all
 // timed side by side: 32 rows per warp (x shared, half the warps: 51.5 against 44.8); more warps by fewer
@@ -167,48 +167,50 @@ __device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_out(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void store_out(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// kTiles groups of eight columns; kBytes weight bytes per thread, row and step (a step is 8 * kBytes
+// kTiles groups of eight columns; kHeight times 16 rows of weights per warp; kBytes weight bytes per thread, row and step (a step is 8 * kBytes
 // values of K: it has to lie inside a group).
-template <typename T, int kTiles, int kBytes>
+template <typename T, int kTiles, int kBytes, int kHeight>
 __global__ void __launch_bounds__(kWarps * 32) matvec_w4_kernel(const W4Args a) {
   constexpr int kParts = sizeof(T) == 4 ? 3 : 1;   // columns per row of x
   constexpr int kStep = 8 * kBytes;
-  __shared__ float sums[kWarps][16][8 * kTiles + 1];
+  __shared__ float sums[kWarps][16 * kHeight][8 * kTiles + 1];
+  constexpr int kRows = 2 * kHeight;   // weight rows per thread, eight apart
   const b200_matvec_w4_problem& q = a.q;
   grid_launch_dependents();
   grid_dependency_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quad = lane >> 2, t = lane & 3;
-  const int row0 = blockIdx.x * 16;
+  const int row0 = blockIdx.x * 16 * kHeight;
   const int groups = a.groups, group_steps = a.group_steps, steps = a.steps;
   const int begin = static_cast<int>(static_cast<int64_t>(steps) * warp / kWarps), end = static_cast<int>(static_cast<int64_t>(steps) * (warp + 1) / kWarps);
-  // This thread's two weight rows. Rows behind the last are read as the last one and not stored.
-  const uint8_t* w[2];
-  int64_t at[2];   // of the group's scale and zero
+  // This thread's weight rows. Rows behind the last are read as the last one and not stored.
+  const uint8_t* w[kRows];
+  int64_t at[kRows];   // of the group's scale and zero
   const int group = group_steps == 1 ? begin : begin / group_steps;
   int left = (group + 1) * group_steps - begin;   // steps left in the group
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < kRows; ++i) {
     const int64_t r = min(row0 + 8 * i + quad, q.n - 1);
     w[i] = q.qweight + r * (q.k / 2) + t * kBytes + static_cast<int64_t>(begin) * (kStep / 2);
     at[i] = r * groups + group;
   }
 
-  float total[kTiles][4] = {};
-  float scale[2];
-  ZeroPair zero[2];
+  float total[kHeight][kTiles][4] = {};
+  float scale[kRows];
+  ZeroPair zero[kRows];
   uint32_t base;   // a register that the compiler takes for no constant, which would cost an instruction per use
   asm volatile("mov.b32 %0, %1;" : "=r"(base) : "n"(Pair<T>::kBase));
-  zero[0] = zero[1] = zero_pair<T>(8);
-  bool fresh = true;
-#pragma unroll 2
-  for (int s = begin; s < end; ++s) {
-    Packed<kBytes> p[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) p[i].load(w[i]), w[i] += kStep / 2;
+  for (int i = 0; i < kRows; ++i) zero[i] = zero_pair<T>(8);
+  bool fresh = true;
+#pragma unroll(kHeight == 1 ? 2 : 1)
+  for (int s = begin; s < end; ++s) {
+    Packed<kBytes> p[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) p[i].load(w[i]), w[i] += kStep / 2;
     if (fresh) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < kRows; ++i) {
         scale[i] = scale_at(q.scales, q.scale_dtype, at[i]);
         if (q.zeros != nullptr) zero[i] = zero_pair<T>(__ldg(q.zeros + at[i]) & 15u);
         ++at[i];
@@ -216,37 +218,43 @@ __global__ void __launch_bounds__(kWarps * 32) matvec_w4_kernel(const W4Args a) 
     }
     fresh = --left == 0;
     if (fresh) left = group_steps;
-    float acc[kTiles][4] = {};
+    float acc[kHeight][kTiles][4] = {};
 #pragma unroll
     for (int i = 0; i < kBytes / 4; ++i) {
-      uint32_t m[2][4];
+      uint32_t m[kRows][4];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) decode<T>(m[r], p[r].w[i], zero[r], base);
-      const uint32_t first[4] = {m[0][0], m[1][0], m[0][1], m[1][1]}, second[4] = {m[0][2], m[1][2], m[0][3], m[1][3]};
+      for (int r = 0; r < kRows; ++r) decode<T>(m[r], p[r].w[i], zero[r], base);
       const int64_t k = static_cast<int64_t>(s) * kStep + t * 2 * kBytes + i * 8;
 #pragma unroll
       for (int c = 0; c < kTiles; ++c) {
         const int column = c * 8 + quad;
         uint32_t x[4] = {0, 0, 0, 0};
         if (column < q.rows * kParts) load_pairs<T>(x, static_cast<const T*>(q.x) + static_cast<int64_t>(column / kParts) * q.k + k, column % kParts);
-        Pair<T>::mma(acc[c], first, x[0], x[1]);
-        Pair<T>::mma(acc[c], second, x[2], x[3]);
+#pragma unroll
+        for (int h = 0; h < kHeight; ++h) {
+          const uint32_t(&upper)[4] = m[2 * h], (&lower)[4] = m[2 * h + 1];
+          const uint32_t first[4] = {upper[0], lower[0], upper[1], lower[1]}, second[4] = {upper[2], lower[2], upper[3], lower[3]};
+          Pair<T>::mma(acc[h][c], first, x[0], x[1]);
+          Pair<T>::mma(acc[h][c], second, x[2], x[3]);
+        }
       }
     }
 #pragma unroll
-    for (int c = 0; c < kTiles; ++c) {
-      total[c][0] += scale[0] * acc[c][0], total[c][1] += scale[0] * acc[c][1];
-      total[c][2] += scale[1] * acc[c][2], total[c][3] += scale[1] * acc[c][3];
-    }
+    for (int h = 0; h < kHeight; ++h)
+#pragma unroll
+      for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) total[h][c][e] += scale[2 * h + e / 2] * acc[h][c][e];
   }
 #pragma unroll
-  for (int c = 0; c < kTiles; ++c) {
-    sums[warp][quad][c * 8 + 2 * t] = total[c][0], sums[warp][quad][c * 8 + 2 * t + 1] = total[c][1];
-    sums[warp][quad + 8][c * 8 + 2 * t] = total[c][2], sums[warp][quad + 8][c * 8 + 2 * t + 1] = total[c][3];
-  }
+  for (int h = 0; h < kHeight; ++h)
+#pragma unroll
+    for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sums[warp][16 * h + 8 * (e / 2) + quad][c * 8 + 2 * t + e % 2] = total[h][c][e];
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * q.rows; i += kWarps * 32) {
-    const int n = i % 16, m = i / 16;
+  for (int i = threadIdx.x; i < 16 * kHeight * q.rows; i += kWarps * 32) {
+    const int n = i % (16 * kHeight), m = i / (16 * kHeight);
     if (row0 + n >= q.n) continue;
     float sum = 0.f;
     for (int v = 0; v < kWarps; ++v)
@@ -256,17 +264,32 @@ __global__ void __launch_bounds__(kWarps * 32) matvec_w4_kernel(const W4Args a) 
   }
 }
 
-template <typename T, int kTiles, int kBytes>
-int launch(const b200_matvec_w4_problem& q, cudaStream_t s) {
+template <typename T, int kTiles, int kBytes, int kHeight>
+int launch_height(const b200_matvec_w4_problem& q, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(q.n) + 15) / 16));
+  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(q.n) + 16 * kHeight - 1) / (16 * kHeight)));
   cfg.blockDim = dim3(kWarps * 32);
   cfg.stream = s;
   const GemmLaunchAttributes attrs = gemm_launch_attributes(1);
   cfg.attrs = const_cast<cudaLaunchAttribute*>(attrs.list);
   cfg.numAttrs = attrs.count;
-  if (cudaLaunchKernelEx(&cfg, matvec_w4_kernel<T, kTiles, kBytes>, W4Args{q, q.k / q.group, q.k / (8 * kBytes), q.group / (8 * kBytes)}) != cudaSuccess) return launch_failed();
+  if (cudaLaunchKernelEx(&cfg, matvec_w4_kernel<T, kTiles, kBytes, kHeight>, W4Args{q, q.k / q.group, q.k / (8 * kBytes), q.group / (8 * kBytes)}) != cudaSuccess) return launch_failed();
   return launch_status();
+}
+
+// Warps of 32 rows of weights read x half as often, but there are half as many of them. That pays when x
+// is what a CTA mostly reads, from L2: with six columns or more, and two CTAs left for every
+// multiprocessor. BF16 by 28672 x 8192, 32 against 16 rows: 47 and 58 us of 8 rows, 72 and 93 of 16, but
+// 43 and 39 of 4; 8 rows by 4096 x 4096 13.3 and 10.8. Short runs of codes (groups of 64) lose with
+// 16-bit x (19.9 and 18.0 of 8 rows by 14336 x 4096); FP32 x, three times as much work, gains (69 and 122).
+template <typename T, int kTiles, int kBytes>
+int launch(const b200_matvec_w4_problem& q, cudaStream_t s) {
+  constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
+  if constexpr (kTiles <= 3 && kBytes >= (kParts == 3 ? 8 : 16)) {
+    constexpr int kLarge = 2 * 148 * 32;
+    if (q.rows * kParts >= 6 && q.n >= kLarge) return launch_height<T, kTiles, kBytes, 2>(q, s);
+  }
+  return launch_height<T, kTiles, kBytes, 1>(q, s);
 }
 
 template <typename T, int kTiles>

@@ -380,6 +380,14 @@ def test_matvec_w4(dtype, rows, n, k, group, zeros):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n,k,group,zeros", [(6, 9472, 256, 128, True), (8, 9473, 384, 128, True), (16, 10001, 128, 128, False),
+                                                  (5, 9999, 192, 64, True), (2, 9503, 1152, 128, False), (9, 9488, 96, 32, True)])
+def test_matvec_w4_many_weight_rows(dtype, rows, n, k, group, zeros):
+    x, qweight, scales, z = w4_inputs(19, rows, n, k, group, dtype, zeros)
+    check_w4(K.matvec_w4(x, qweight, scales, z), x, qweight, scales, z)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_matvec_w4_every_code_and_position(dtype):
     # Unit rows of x read single weights: every nibble has to come out where it was put in.
     k, n = 128, 16
