@@ -39,7 +39,6 @@
 namespace b200 {
 namespace {
 
-constexpr int kWarps = 8;
 constexpr int kMaxRows = 16;
 
 struct W4Args {
@@ -169,7 +168,7 @@ __device__ __forceinline__ void store_out(__nv_bfloat16* p, float v) { *p = __fl
 
 // kTiles groups of eight columns; kHeight times 16 rows of weights per warp; kBytes weight bytes per thread, row and step (a step is 8 * kBytes
 // values of K: it has to lie inside a group).
-template <typename T, int kTiles, int kBytes, int kHeight>
+template <typename T, int kTiles, int kBytes, int kHeight, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32) matvec_w4_kernel(const W4Args a) {
   constexpr int kParts = sizeof(T) == 4 ? 3 : 1;   // columns per row of x
   constexpr int kStep = 8 * kBytes;
@@ -264,8 +263,8 @@ __global__ void __launch_bounds__(kWarps * 32) matvec_w4_kernel(const W4Args a) 
   }
 }
 
-template <typename T, int kTiles, int kBytes, int kHeight>
-int launch_height(const b200_matvec_w4_problem& q, cudaStream_t s) {
+template <typename T, int kTiles, int kBytes, int kHeight, int kWarps>
+int launch_shape(const b200_matvec_w4_problem& q, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(q.n) + 16 * kHeight - 1) / (16 * kHeight)));
   cfg.blockDim = dim3(kWarps * 32);
@@ -273,7 +272,7 @@ int launch_height(const b200_matvec_w4_problem& q, cudaStream_t s) {
   const GemmLaunchAttributes attrs = gemm_launch_attributes(1);
   cfg.attrs = const_cast<cudaLaunchAttribute*>(attrs.list);
   cfg.numAttrs = attrs.count;
-  if (cudaLaunchKernelEx(&cfg, matvec_w4_kernel<T, kTiles, kBytes, kHeight>, W4Args{q, q.k / q.group, q.k / (8 * kBytes), q.group / (8 * kBytes)}) != cudaSuccess) return launch_failed();
+  if (cudaLaunchKernelEx(&cfg, matvec_w4_kernel<T, kTiles, kBytes, kHeight, kWarps>, W4Args{q, q.k / q.group, q.k / (8 * kBytes), q.group / (8 * kBytes)}) != cudaSuccess) return launch_failed();
   return launch_status();
 }
 
@@ -287,9 +286,22 @@ int launch(const b200_matvec_w4_problem& q, cudaStream_t s) {
   constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
   if constexpr (kTiles <= 3 && kBytes >= (kParts == 3 ? 8 : 16)) {
     constexpr int kLarge = 2 * 148 * 32;
-    if (q.rows * kParts >= 6 && q.n >= kLarge) return launch_height<T, kTiles, kBytes, 2>(q, s);
+    if (q.rows * kParts >= 6 && q.n >= kLarge) return launch_shape<T, kTiles, kBytes, 2, 8>(q, s);
   }
-  return launch_height<T, kTiles, kBytes, 1>(q, s);
+  // Few CTAs: as many warps in each as leave all CTAs room at once, one or two per multiprocessor. 16
+  // against 8 warps, BF16: one row by 4096 x 4096 5.7 and 8.3 us, by 4096 x 14336 12.1 and 22.6, 16 rows
+  // by 2048 x 8192 9.0 and 18.7. Two CTAs of 16 warps have 64 registers per thread, which only 16-bit x of
+  // up to eight rows does with; else 12 warps (16 rows by 4096 x 14336 23.3, 8 warps 34.1, 16 24.5).
+  // More CTAs than that lose by it (16 rows by 5120 x 5120 13.5 with 8 warps, 18.9 with 12).
+  if constexpr (kTiles <= 3) {
+    constexpr bool kSmall = kTiles == 1 && kParts == 1;
+    constexpr int kRound = 148 * 16;   // rows of one CTA per multiprocessor
+    if (q.n <= (kSmall ? 2 * kRound : kRound)) return launch_shape<T, kTiles, kBytes, 1, 16>(q, s);
+    if constexpr (!kSmall) {
+      if (q.n <= 2 * kRound) return launch_shape<T, kTiles, kBytes, 1, 12>(q, s);
+    }
+  }
+  return launch_shape<T, kTiles, kBytes, 1, 8>(q, s);
 }
 
 template <typename T, int kTiles>

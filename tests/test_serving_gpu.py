@@ -381,7 +381,10 @@ def test_matvec_w4(dtype, rows, n, k, group, zeros):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,n,k,group,zeros", [(6, 9472, 256, 128, True), (8, 9473, 384, 128, True), (16, 10001, 128, 128, False),
-                                                  (5, 9999, 192, 64, True), (2, 9503, 1152, 128, False), (9, 9488, 96, 32, True)])
+                                                  (5, 9999, 192, 64, True), (2, 9503, 1152, 128, False), (9, 9488, 96, 32, True),
+                                                  # around the sizes from which a CTA has fewer warps
+                                                  (1, 4736, 2176, 128, True), (8, 4737, 192, 64, False), (3, 2368, 160, 32, True),
+                                                  (16, 2369, 384, 128, True), (7, 4725, 2048, 256, False), (12, 2300, 1088, 64, True)])
 def test_matvec_w4_many_weight_rows(dtype, rows, n, k, group, zeros):
     x, qweight, scales, z = w4_inputs(19, rows, n, k, group, dtype, zeros)
     check_w4(K.matvec_w4(x, qweight, scales, z), x, qweight, scales, z)
