@@ -4,7 +4,6 @@ Four operators of one serving step of a decoder: attention over packed prompts, 
 that shares a prefix, the matrix-vector product with 4-bit weights, and the processing of logits before the
 softmax. `own` chooses between the calls of the package (true) and elementary torch operations (false).
 """
-import functools
 import math
 import sys
 from pathlib import Path
@@ -191,17 +190,12 @@ def run(state):
     return {"prompt": _plain_prompt, "shared": _plain_shared, "matvec": _plain_matvec, "logits": _plain_logits}[state["case"]["op"]](state)
 
 
-@functools.cache
-def _package():
-    """The package, found and imported once, as by a program's import statement."""
-    sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "cuda-ai-infra-kernels_b200" / "python"))
-    import cuda_ai_kernels
-
-    return cuda_ai_kernels
-
-
 def _own(s):
-    K = _package()
+    package = str(Path(__file__).resolve().parents[1] / "cuda-ai-infra-kernels_b200" / "python")
+    if package not in sys.path:
+        sys.path.insert(0, package)
+    import cuda_ai_kernels as K
+
     op = s["case"]["op"]
     if op == "prompt":
         return K.attention_prompt(s["q"], s["k"], s["v"], s["cu_q"], s["cu_k"])
