@@ -222,10 +222,11 @@ Plan plan(AttentionArgs* a) {
     ranges = (prefix * longest + own * blocks(a->room)) * a->kv_heads;
     most = (ranges << a->pair_shift) + (prefix + own) * a->kv_heads * a->unit_cost;
   } else {
-    // Each sequence, and the rows behind them, rounds up once.
+    // Each sequence, and the rows in front of them and behind them, rounds up once. (A call has rows in
+    // front only where its first offset is not zero: they are not counted on for the grid.)
     const int64_t all = (static_cast<int64_t>(a->q_rows) * a->group / a->unit_rows + a->sequences + 1) * a->kv_heads;
     ranges = all * (longest > 0 ? longest : 1);
-    most = all * ((longest << a->pair_shift) + a->unit_cost);
+    most = (all + a->kv_heads) * ((longest << a->pair_shift) + a->unit_cost);
   }
   // On the device the line is counted in 32 bits; it would take minutes to work through.
   if (most > 0x7fffffff) return {B200_ERR_INVALID_PROBLEM, false};

@@ -2,9 +2,9 @@
 // partial results (attention.cu).
 //
 // Both operators are lists of sequences: n query tokens that see m keys. A prompt call has one per
-// packed sequence (and a last one for the rows behind them, which sees nothing); a shared-prefix
-// call has the whole batch over the prefix first and then every request over its own part of the
-// cache. The rows of a key head are (token, query head of its group) pairs in that order, row
+// packed sequence (and then one for the rows behind them and one for the rows in front of them, which
+// see nothing); a shared-prefix call has the whole batch over the prefix first and then every request
+// over its own part of the cache. The rows of a key head are (token, query head of its group) pairs in that order, row
 // i * group + g, so that all rows that read the same keys sit side by side whatever the head layout
 // is: a decoding batch fills a tile with requests and heads as a prompt fills it with tokens.
 //
@@ -39,7 +39,7 @@ struct AttentionArgs {
   void* out;
   const int32_t *cu_q, *cu_k, *lengths;
   int kind, dtype;
-  int sequences;                     // prompt: without the rows behind the last one; shared: 1 + batch
+  int sequences;                     // prompt: without the rows in front and behind; shared: 1 + batch
   int q_rows, k_rows, room;          // k_rows: keys of the packed array, or of the prefix
   int heads, kv_heads, group, dim;
   float scale_log2;                  // scale * log2(e): exponentials are powers of two
@@ -81,7 +81,7 @@ inline int log2_or_minus_one(int v) {
 
 __host__ __device__ inline int clamp_int(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
 
-__device__ __forceinline__ int sequence_count(const AttentionArgs& a) { return a.sequences + (a.kind == kPrompt ? 1 : 0); }
+__device__ __forceinline__ int sequence_count(const AttentionArgs& a) { return a.sequences + (a.kind == kPrompt ? 2 : 0); }
 
 __device__ __forceinline__ Sequence sequence_of(const AttentionArgs& a, int s) {
   Sequence r{};
@@ -94,9 +94,15 @@ __device__ __forceinline__ Sequence sequence_of(const AttentionArgs& a, int s) {
     }
     return r;
   }
-  const int next = min(s + 1, a.sequences);   // all four on their way at once
-  const int q0 = __ldg(a.cu_q + s), q1 = __ldg(a.cu_q + next), k0 = __ldg(a.cu_k + s), k1 = __ldg(a.cu_k + next);
-  r.q_row = clamp_int(q0, 0, a.q_rows);
+  const bool front = s > a.sequences;
+  const int from = front ? 0 : s, next = min(s + 1, a.sequences);   // all four on their way at once
+  const int q0 = __ldg(a.cu_q + from), q1 = __ldg(a.cu_q + next), k0 = __ldg(a.cu_k + from), k1 = __ldg(a.cu_k + next);
+  const int first = clamp_int(q0, 0, a.q_rows);
+  if (front) {
+    r.n = first;
+    return r;
+  }
+  r.q_row = first;
   r.k_row = clamp_int(k0, 0, a.k_rows);
   if (s == a.sequences) {
     r.n = a.q_rows - r.q_row;

@@ -141,11 +141,11 @@ def attention_prompt(
     ``m - n + i + 1`` when ``causal`` (a chunk of a prompt, or a single token, at the end
     of its cached keys), else all. ``scale`` defaults to ``dim ** -0.5``.
 
-    Rows that see no key, and rows behind the last sequence, are zero. Types: float32
-    (FP32 arithmetic), float16, bfloat16 (tensor cores, FP32 sums). ``dim`` is a multiple
-    of 8 up to 128. Strided views are taken as they are where their rows sit on 16-byte
-    granules, and copied otherwise. Keys and values outside a sequence may hold anything;
-    inside one, ``v`` must be finite.
+    Rows that see no key, and rows in front of the first sequence or behind the last, are
+    zero. Types: float32 (FP32 arithmetic), float16, bfloat16 (tensor cores, FP32 sums).
+    ``dim`` is a multiple of 8 up to 128. Strided views are taken as they are where their
+    rows sit on 16-byte granules, and copied otherwise. Keys and values outside a sequence
+    may hold anything; inside one, ``v`` must be finite.
     """
     return _C.attention_prompt(q, k, v, cu_seqlens_q, cu_seqlens_k, causal, scale)
 

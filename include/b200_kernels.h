@@ -358,9 +358,9 @@ typedef struct b200_rows_view {
  * key head h / (heads / kv_heads). With n queries and m keys, and `causal` set,
  * query i sees the keys j <= i + m - n (the last query sees all of them):
  *   out_i = sum_j p_ij v_j,  p_i = softmax over the visible j of scale * q_i . k_j.
- * A row that sees no key is zero; so are the rows behind cu_q[sequences]. What lies
- * in keys or values outside a sequence is never read into its result, NaN and
- * infinities included. Inside a sequence, V must be finite.
+ * A row that sees no key is zero; so are the rows in front of cu_q[0] and behind
+ * cu_q[sequences]. What lies in keys or values outside a sequence is never read into
+ * its result, NaN and infinities included. Inside a sequence, V must be finite.
  *   dim: a multiple of 8, 8 .. 128; heads / kv_heads <= 128; scale > 0.
  *   FP16 / BF16 run on the tensor cores (probabilities rounded to the operand type
  *   for the second product, all sums in FP32); FP32 runs on the FMA pipe.
