@@ -214,22 +214,27 @@ Plan plan(AttentionArgs* a) {
   const auto blocks = [&](int64_t rows) { return (rows + keys - 1) / keys; };
   const auto units = [&](int64_t rows) { return (rows + a->unit_rows - 1) / a->unit_rows; };
   const int64_t longest = blocks(a->k_rows);
-  int64_t most;        // length of the line
-  int64_t ranges;      // more CTAs than this would have nothing to do
+  __int128 most;       // length of the line
+  __int128 ranges;     // more CTAs than this would have nothing to do
   if (a->kind == kShared) {
     if (a->kv_heads > 65535) return {B200_ERR_INVALID_PROBLEM, false};   // a dimension of the join's grid
-    const int64_t prefix = units(static_cast<int64_t>(a->q_rows) * a->group), own = a->q_rows;
+    const __int128 prefix = units(static_cast<int64_t>(a->q_rows) * a->group), own = a->q_rows;
     ranges = (prefix * longest + own * blocks(a->room)) * a->kv_heads;
     most = (ranges << a->pair_shift) + (prefix + own) * a->kv_heads * a->unit_cost;
   } else {
     // Each sequence, and the rows in front of them and behind them, rounds up once. (A call has rows in
     // front only where its first offset is not zero: they are not counted on for the grid.)
-    const int64_t all = (static_cast<int64_t>(a->q_rows) * a->group / a->unit_rows + a->sequences + 1) * a->kv_heads;
-    ranges = all * (longest > 0 ? longest : 1);
-    most = (all + a->kv_heads) * ((longest << a->pair_shift) + a->unit_cost);
+    const __int128 whole = a->q_rows / a->tokens, all = whole + a->sequences + 1;
+    ranges = all * a->kv_heads * (longest > 0 ? longest : 1);
+    // A sequence of n queries and m keys has at most n / tokens + 1 units of m / keys + 1 blocks. Summed
+    // over sequences that do not overlap: n m to at most all queries by all keys, n and m to all of them.
+    const __int128 all_keys = a->k_rows / keys + 1;
+    most = ((((whole + 1) * all_keys + whole + 1 + all_keys + a->sequences) << a->pair_shift) + (all + 1) * a->unit_cost) * a->kv_heads;
   }
-  // On the device the line is counted in 32 bits; it would take minutes to work through.
-  if (most > 0x7fffffff) return {B200_ERR_INVALID_PROBLEM, false};
+  // On the device the line is counted in 64 bits, with room for a sum per thread. It would take years to
+  // work through.
+  if (most >= __int128{1} << 54) return {B200_ERR_INVALID_PROBLEM, false};
+  a->longest_line = static_cast<int64_t>(most);
   if (ranges < a->ctas) a->ctas = static_cast<int>(ranges > 0 ? ranges : 1);
   return {B200_OK, a->kind == kShared || longest > 1};   // units of one block are never cut
 }

@@ -17,6 +17,9 @@
 // partial result (sum, maximum, denominator) per CTA that worked on it, and a second launch joins
 // them in CTA order: at most one unit per boundary, so the traffic does not grow with the call. In a
 // shared-prefix call every row has two units, one per part of its keys, and all results are partial.
+// Positions on the line are of type Line: 32 bits, or 64 where the arrays are large enough for a line that
+// passes them (a million causal tokens of 64 heads). With 64 throughout, the segment walk's registers
+// and divisions cost 64 requests behind a prefix 10 of 112 us and ragged prompts 6 of 119.
 // Lengths are read on the device only. Offsets and lengths are clamped to the arrays here.
 #pragma once
 
@@ -49,6 +52,7 @@ struct AttentionArgs {
   int token_shift;                   // its logarithm where it is a power of two, else -1
   int unit_cost, pair_shift;         // on the line: of a unit; logarithm of a block's for a unit of more than half the rows
   int ctas;                          // ranges
+  int64_t longest_line;              // that sequences which do not overlap can make
   // Partial results, in slots of some rows: maximum (scaled, base 2) and denominator [row], and the sum,
   // not divided by it, as [dim / 4][row][4], so that the threads of a warp, which own one row
   // each, write and read whole lines. First the slots of units continued from the CTA before,
@@ -158,24 +162,23 @@ static __device__ __noinline__ int64_t floor_sum(int n, int m, int a, int b) {
   return sum;
 }
 
-// Length of the first `units` of the `all` units of one key head of the sequence. The launcher has made
-// sure that the whole line fits 32 bits. Not inlined: a CTA calls it three or four times as it starts,
+// Length of the first `units` of the `all` units of one key head of the sequence. Not inlined: a CTA calls it three or four times as it starts,
 // when every instruction has to be fetched before it runs.
-template <int kKeys>
-__device__ __noinline__ int length_before(const AttentionArgs& a, const Sequence& s, int units, int all) {
+template <int kKeys, typename Line>
+__device__ __noinline__ Line length_before(const AttentionArgs& a, const Sequence& s, int units, int all) {
   if (units == 0) return 0;
   const int regular = units < all ? units : all - 1;   // all but the last have all their rows
   const int rest = units == all ? unit_length<kKeys>(a, s, all - 1) : 0;
-  if (a.kind == kShared || a.causal == 0) return (regular > 0 ? regular * unit_length<kKeys>(a, s, 0) : 0) + rest;
+  if (a.kind == kShared || a.causal == 0) return (regular > 0 ? static_cast<Line>(regular) * unit_length<kKeys>(a, s, 0) : 0) + rest;
   // Unit t holds whole tokens; but for the last of all, its last token sees c + tokens * (t + 1) keys.
   const int tokens = a.tokens, c = s.m - s.n;
   const int blind = c >= 0 ? 0 : min(-c / tokens, regular);   // units that see nothing
   const int n = regular - blind, b = c + tokens * (blind + 1) + kKeys - 1;
-  int sum = 0;   // blocks
+  Line sum = 0;   // blocks
   if (a.token_shift < 0) {
-    sum += static_cast<int>(floor_sum(n, kKeys, tokens, b));
+    sum += static_cast<Line>(floor_sum(n, kKeys, tokens, b));
   } else if (tokens >= kKeys) {
-    sum += static_cast<int>(static_cast<int64_t>(n) * (n - 1) / 2) * (tokens / kKeys) + n * (b / kKeys);
+    sum += static_cast<Line>(static_cast<int64_t>(n) * (n - 1) / 2) * (tokens / kKeys) + static_cast<Line>(n) * (b / kKeys);
   } else {
     // tokens divides the block: floor((tokens i + b) / kKeys) = floor((i + first) / r) with
     // r = kKeys / tokens, first = floor(b / tokens); below x the quotients y / r add up to
@@ -187,53 +190,59 @@ __device__ __noinline__ int length_before(const AttentionArgs& a, const Sequence
       const int q = x >> shift;
       return static_cast<int64_t>(q) * (q - 1) / 2 * (1 << shift) + static_cast<int64_t>(q) * (x - (q << shift));
     };
-    sum += static_cast<int>(below(first + n) - below(first));
+    sum += static_cast<Line>(below(first + n) - below(first));
   }
-  return (sum << a.pair_shift) + regular * a.unit_cost + rest;
+  return (sum << a.pair_shift) + static_cast<Line>(regular) * a.unit_cost + rest;
 }
 
 // ------------------------------------------------------------------------- finding a CTA's work
 
 // Ranges of the line: the first total % ctas are one longer than the rest.
+template <typename Line>
 struct Ranges {
-  int quotient, longer;
-  __device__ __forceinline__ Ranges(int total, int ctas) : quotient(total / ctas), longer(total - quotient * ctas) {}
+  Line quotient;
+  int longer;
+  __device__ __forceinline__ Ranges(Line total, int ctas) : quotient(total / ctas), longer(static_cast<int>(total - quotient * ctas)) {}
   Ranges() = default;
-  __device__ __forceinline__ int begin(int c) const { return c * quotient + min(c, longer); }
-  __device__ __forceinline__ int holder(int position) const {
-    const int boundary = longer * (quotient + 1);
-    return position < boundary ? position / (quotient + 1) : longer + (position - boundary) / quotient;
+  __device__ __forceinline__ Line begin(int c) const { return c * quotient + min(c, longer); }
+  __device__ __forceinline__ int holder(Line position) const {
+    const Line boundary = longer * (quotient + 1);
+    return static_cast<int>(position < boundary ? position / (quotient + 1) : longer + (position - boundary) / quotient);
   }
 };
 
+template <typename Line>
 struct WorkStart {
   int sequence;               // -1: nothing to do
   Sequence seq;
   int units;                  // of a head of the sequence
-  int head, unit, offset;     // offset: into the unit
-  Ranges ranges;
-  int begin, length;          // of this range
+  int head, unit;
+  Line offset;                // into the head's units, and at last into the unit
+  Ranges<Line> ranges;
+  Line begin, length;         // of this range
 };
 
+template <typename Line>
 struct WorkScratch {
   int64_t sums[32];
-  WorkStart start;
+  WorkStart<Line> start;
 };
 
 // Where this CTA's range starts: prefix sums over the sequences by all kThreads threads.
-template <int kKeys, int kThreads>
-__device__ __forceinline__ WorkStart find_range(const AttentionArgs& a, WorkScratch* scratch) {
+template <int kKeys, int kThreads, typename Line>
+__device__ __forceinline__ WorkStart<Line> find_range(const AttentionArgs& a, WorkScratch<Line>* scratch) {
   const int count = sequence_count(a);
   const int chunk = (count + kThreads - 1) / kThreads;
   const int lo = min(static_cast<int>(threadIdx.x) * chunk, count), hi = min(lo + chunk, count);
   Sequence seq{};
-  int size = 0;
-  int64_t mine = 0;   // offsets that overlap could make the line longer than the launcher counted on
+  Line size = 0;
+  int64_t mine = 0;   // sequences that overlap could make the line longer than the launcher counted on
   for (int s = lo; s < hi; ++s) {
     seq = sequence_of(a, s);
     const int units = unit_count(a, seq);
-    size = a.kv_heads * length_before<kKeys>(a, seq, units, units);
+    size = a.kv_heads * length_before<kKeys, Line>(a, seq, units, units);
     mine += size;
+    if (sizeof(Line) == 8) mine = min(mine, a.longest_line + 1);   // of 2^30 sequences the sum would pass 64 bits
   }
   int64_t upto = mine;   // inclusive over the warp
 #pragma unroll
@@ -242,7 +251,7 @@ __device__ __forceinline__ WorkStart find_range(const AttentionArgs& a, WorkScra
     if ((threadIdx.x & 31) >= o) upto += other;
   }
   if ((threadIdx.x & 31) == 31) scratch->sums[threadIdx.x >> 5] = upto;
-  WorkStart& start = scratch->start;
+  WorkStart<Line>& start = scratch->start;
   if (threadIdx.x == 0) start.sequence = -1;
   __syncthreads();
   int64_t ahead = upto - mine, whole = 0;
@@ -250,26 +259,27 @@ __device__ __forceinline__ WorkStart find_range(const AttentionArgs& a, WorkScra
     if (w < static_cast<int>(threadIdx.x >> 5)) ahead += scratch->sums[w];
     whole += scratch->sums[w];
   }
-  const int total = whole <= 0x7fffffff ? static_cast<int>(whole) : 0;   // too long: nothing is done
-  int before = static_cast<int>(min(ahead, static_cast<int64_t>(total)));
-  const Ranges ranges(total, a.ctas);
-  const int begin = ranges.begin(blockIdx.x), length = ranges.begin(blockIdx.x + 1) - begin;
+  const Line total = whole <= a.longest_line ? static_cast<Line>(whole) : 0;   // too long: nothing is done
+  Line before = static_cast<Line>(min(ahead, static_cast<int64_t>(total)));
+  const Ranges<Line> ranges(total, a.ctas);
+  const Line begin = ranges.begin(blockIdx.x), length = ranges.begin(blockIdx.x + 1) - begin;
   if (length > 0 && begin >= before && begin < ahead + mine) {
     int s = lo;
     if (hi - lo > 1) {
       for (; s < hi; ++s) {
         seq = sequence_of(a, s);
         const int units = unit_count(a, seq);
-        size = a.kv_heads * length_before<kKeys>(a, seq, units, units);
+        size = a.kv_heads * length_before<kKeys, Line>(a, seq, units, units);
         if (begin < before + size) break;
         before += size;
       }
     }
-    const int per_head = size / a.kv_heads, head = (begin - before) / per_head;
-    start = WorkStart{s, seq, unit_count(a, seq), head, 0, begin - before - head * per_head, ranges, begin, length};
+    const Line per_head = size / a.kv_heads;
+    const int head = static_cast<int>((begin - before) / per_head);
+    start = WorkStart<Line>{s, seq, unit_count(a, seq), head, 0, begin - before - head * per_head, ranges, begin, length};
   }
   __syncthreads();
-  WorkStart found = start;
+  WorkStart<Line> found = start;
   if (found.sequence < 0) return found;
   // The last unit that does not start behind the position, by all threads at once.
   int low = 0, high = found.units;
@@ -278,8 +288,8 @@ __device__ __forceinline__ WorkStart find_range(const AttentionArgs& a, WorkScra
     const int mid = low + step * static_cast<int>(threadIdx.x), end = min(mid + step, high);
     __syncthreads();
     if (mid < high) {
-      const int first = length_before<kKeys>(a, found.seq, mid, found.units);
-      if (first <= found.offset && (end == high || found.offset < length_before<kKeys>(a, found.seq, end, found.units)))
+      const Line first = length_before<kKeys, Line>(a, found.seq, mid, found.units);
+      if (first <= found.offset && (end == high || found.offset < length_before<kKeys, Line>(a, found.seq, end, found.units)))
         start.unit = mid, start.offset = found.offset - first;
     }
     __syncthreads();
@@ -298,25 +308,25 @@ struct Segment {
 };
 
 // Walks the segments of a CTA's range.
-template <int kKeys>
+template <int kKeys, typename Line>
 struct SegmentWalk {
   const AttentionArgs& a;
-  Ranges ranges;
-  int position, end;   // on the line
+  Ranges<Line> ranges;
+  Line position, end;   // on the line
   int sequence, units;
   Sequence seq;
   int head, unit, offset;
 
-  __device__ __forceinline__ SegmentWalk(const AttentionArgs& args, const WorkStart& start) : a(args), ranges(start.ranges) {
+  __device__ __forceinline__ SegmentWalk(const AttentionArgs& args, const WorkStart<Line>& start) : a(args), ranges(start.ranges) {
     position = start.begin, end = start.sequence < 0 ? start.begin : start.begin + start.length;
-    sequence = start.sequence, seq = start.seq, units = start.units, head = start.head, unit = start.unit, offset = start.offset;
+    sequence = start.sequence, seq = start.seq, units = start.units, head = start.head, unit = start.unit, offset = static_cast<int>(start.offset);
   }
 
   __device__ __forceinline__ bool next(Segment* out) {
     while (position < end) {
       const int blocks = unit_blocks<kKeys>(a, seq, unit), length = unit_length<kKeys>(a, seq, unit), shift = block_shift(a, seq, unit);
-      const int from = offset, to = min(length, offset + end - position);
-      const int unit_position = position - from;
+      const int from = offset, to = static_cast<int>(min(static_cast<Line>(length), offset + end - position));
+      const Line unit_position = position - from;
       Segment g{seq, head, unit, max(from - a.unit_cost, 0) >> shift, max(to - a.unit_cost, 0) >> shift, false, false, 0, 0};
       position += to - from;
       offset = to;
@@ -398,6 +408,7 @@ __device__ __forceinline__ int64_t output_row(const AttentionArgs& a, int q_row,
 // each is needed by the join.
 constexpr int kSimtKeyBlock = 64;
 constexpr int kUmmaKeyBlock = 128;
+inline bool wide_line(const AttentionArgs& a) { return a.longest_line > 0x7fffffff; }
 void plan_attention_umma(AttentionArgs* a, int sms);
 void plan_attention_simt(AttentionArgs* a, int sms);
 int launch_attention_umma(const AttentionArgs& a, cudaStream_t s);

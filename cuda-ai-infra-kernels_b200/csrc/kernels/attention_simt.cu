@@ -58,13 +58,13 @@ __device__ __forceinline__ void copy_rows(float* dst, const float* src, int64_t 
 // Four consecutive floats as two pairs.
 __device__ __forceinline__ ulonglong2 pairs_at(const float* p) { return *reinterpret_cast<const ulonglong2*>(p); }
 
-template <int kRows, int kThreads, int kColumns>
+template <int kRows, int kThreads, int kColumns, typename Line>
 __global__ void __launch_bounds__(kThreads, kRows == 16 ? 4 : kRows == 64 ? 2 : 1) attention_simt_kernel(const __grid_constant__ AttentionArgs a) {
   constexpr int kPer = kRows / (kThreads / 16);   // rows of a thread
   constexpr int kQuads = kColumns / 64;           // groups of four of its columns of O
   constexpr int kPitchP = kKeys + 4;
   extern __shared__ __align__(16) float smem[];
-  __shared__ WorkScratch scratch;
+  __shared__ WorkScratch<Line> scratch;
   const int pitch = a.dim + 4;
   float* qs = smem;
   float* ks = qs + kRows * pitch;
@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kThreads, kRows == 16 ? 4 : kRows == 64 ? 2 : 
   grid_launch_dependents();
   grid_dependency_wait();
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  SegmentWalk<kKeys> walk(a, find_range<kKeys, kThreads>(a, &scratch));
+  SegmentWalk<kKeys, Line> walk(a, find_range<kKeys, kThreads, Line>(a, &scratch));
   Segment g;
   if (threadIdx.x == 0) start_records(a);
   while (walk.next(&g)) {
@@ -206,9 +206,9 @@ constexpr size_t simt_smem_bytes(int rows, int dim) {
   return sizeof(float) * ((rows + 2 * static_cast<size_t>(kKeys)) * (dim + 4) + static_cast<size_t>(rows) * (kKeys + 4));
 }
 
-template <int kRows, int kThreads, int kColumns>
-int launch_columns(const AttentionArgs& a, cudaStream_t s) {
-  if (!ensure_dynamic_smem<attention_simt_kernel<kRows, kThreads, kColumns>, simt_smem_bytes(kRows, kColumns)>()) return B200_ERR_LAUNCH_FAILED;
+template <int kRows, int kThreads, int kColumns, typename Line>
+int launch_line(const AttentionArgs& a, cudaStream_t s) {
+  if (!ensure_dynamic_smem<attention_simt_kernel<kRows, kThreads, kColumns, Line>, simt_smem_bytes(kRows, kColumns)>()) return B200_ERR_LAUNCH_FAILED;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.ctas));
   cfg.blockDim = dim3(kThreads);
@@ -217,8 +217,13 @@ int launch_columns(const AttentionArgs& a, cudaStream_t s) {
   const GemmLaunchAttributes attrs = gemm_launch_attributes(1);
   cfg.attrs = const_cast<cudaLaunchAttribute*>(attrs.list);
   cfg.numAttrs = attrs.count;
-  if (cudaLaunchKernelEx(&cfg, attention_simt_kernel<kRows, kThreads, kColumns>, a) != cudaSuccess) return launch_failed();
+  if (cudaLaunchKernelEx(&cfg, attention_simt_kernel<kRows, kThreads, kColumns, Line>, a) != cudaSuccess) return launch_failed();
   return launch_status();
+}
+
+template <int kRows, int kThreads, int kColumns>
+int launch_columns(const AttentionArgs& a, cudaStream_t s) {
+  return wide_line(a) ? launch_line<kRows, kThreads, kColumns, int64_t>(a, s) : launch_line<kRows, kThreads, kColumns, int>(a, s);
 }
 
 template <int kRows, int kThreads>

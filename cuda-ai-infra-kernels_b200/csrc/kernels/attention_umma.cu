@@ -88,7 +88,7 @@ struct Shared {   // behind the tiles
   uint32_t tmem;
   SegmentEntry entries[kEntries];
   float2 exchange[2][kTile];   // maximum and denominator of both streams
-  WorkScratch scratch;
+  WorkScratch<int64_t> scratch;
 };
 constexpr int kEntryReaders = 1 + 2 + 8;
 
@@ -140,12 +140,12 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
 
 // ------------------------------------------------------------------------ segments, value rows
 
-template <int kDim>
-__device__ __forceinline__ void segment_role(const UmmaAttentionArgs& p, const WorkStart& start, uint8_t* smem, Shared* b) {
+template <int kDim, typename Line>
+__device__ __forceinline__ void segment_role(const UmmaAttentionArgs& p, const WorkStart<Line>& start, uint8_t* smem, Shared* b) {
   using S = Smem<kDim>;
   const AttentionArgs& a = p.a;
   const int lane = threadIdx.x & 31;
-  SegmentWalk<kUmmaKeyBlock> walk(a, start);
+  SegmentWalk<kUmmaKeyBlock, Line> walk(a, start);
   Segment g;
   bool ok = true;
   if (lane == 0) start_records(a);
@@ -620,7 +620,7 @@ __device__ __forceinline__ void softmax_role(const UmmaAttentionArgs& p, Shared*
   }
 }
 
-template <int kDim, bool kBf16>
+template <int kDim, bool kBf16, typename Line>
 __global__ void __launch_bounds__(kThreads, 1) attention_umma_kernel(const __grid_constant__ UmmaAttentionArgs p) {
   using S = Smem<kDim>;
   extern __shared__ __align__(1024) uint8_t smem[];   // the swizzle's period
@@ -651,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_umma_kernel(const __gri
   const uint32_t tmem = b.tmem;
   grid_launch_dependents();   // after the allocation: a following kernel may want tensor memory too
   grid_dependency_wait();
-  const WorkStart start = find_range<kUmmaKeyBlock, kThreads>(p.a, &b.scratch);
+  const WorkStart<Line> start = find_range<kUmmaKeyBlock, kThreads, Line>(p.a, reinterpret_cast<WorkScratch<Line>*>(&b.scratch));
   if (warp < 8) {
     registers_raise<kSoftmaxRegisters>();
     softmax_role<kBf16, S::kSlots>(p, &b, smem + S::kStaging, tmem);
@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_umma_kernel(const __gri
     registers_lower<kOtherRegisters>();
     if (warp == 8 && lane == 0) copy_role<kDim>(p, smem, &b);
     if ((warp == 9 || warp == 10) && lane == 0) MmaIssuer<kDim, kBf16>(p.a, smem, &b, tmem, warp - 9).run();
-    if (warp == 11) segment_role<kDim>(p, start, smem, &b);
+    if (warp == 11) segment_role<kDim, Line>(p, start, smem, &b);
   }
   __syncwarp();
   tcgen05_fence_before_sync();
@@ -668,11 +668,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_umma_kernel(const __gri
   if (warp == 9) tmem_dealloc<512>(tmem);
 }
 
-template <int kDim, bool kBf16>
-int launch(const UmmaAttentionArgs& p, cudaStream_t s) {
+template <int kDim, bool kBf16, typename Line>
+int launch_line(const UmmaAttentionArgs& p, cudaStream_t s) {
   constexpr size_t kBytes = Smem<kDim>::kTiles + sizeof(Shared);
   static_assert(kBytes <= 227 * 1024, "shared memory of one CTA");
-  if (!ensure_dynamic_smem<attention_umma_kernel<kDim, kBf16>, kBytes>()) return B200_ERR_LAUNCH_FAILED;
+  if (!ensure_dynamic_smem<attention_umma_kernel<kDim, kBf16, Line>, kBytes>()) return B200_ERR_LAUNCH_FAILED;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.a.ctas));
   cfg.blockDim = dim3(kThreads);
@@ -681,8 +681,13 @@ int launch(const UmmaAttentionArgs& p, cudaStream_t s) {
   const GemmLaunchAttributes attrs = gemm_launch_attributes(1);
   cfg.attrs = const_cast<cudaLaunchAttribute*>(attrs.list);
   cfg.numAttrs = attrs.count;
-  if (cudaLaunchKernelEx(&cfg, attention_umma_kernel<kDim, kBf16>, p) != cudaSuccess) return launch_failed();
+  if (cudaLaunchKernelEx(&cfg, attention_umma_kernel<kDim, kBf16, Line>, p) != cudaSuccess) return launch_failed();
   return launch_status();
+}
+
+template <int kDim, bool kBf16>
+int launch(const UmmaAttentionArgs& p, cudaStream_t s) {
+  return wide_line(p.a) ? launch_line<kDim, kBf16, int64_t>(p, s) : launch_line<kDim, kBf16, int>(p, s);
 }
 
 // [rows][heads][dim] as (dim, heads, rows, batch); a box is one head's 128 rows, 64 columns.

@@ -368,6 +368,7 @@ typedef struct b200_rows_view {
  *   (B200_ERR_MISALIGNED_OPERAND otherwise); out is dense [tokens][heads][dim].
  * cu_q and cu_k are device arrays of sequences + 1 offsets; they are read by the
  * kernels only, and offsets outside the arrays do not lead to accesses outside them.
+ * B200_ERR_INVALID_PROBLEM: rows, or query rows times heads / kv_heads, above 2^30.
  * `workspace` (16-byte aligned, b200_attention_prompt_workspace_bytes) holds partial
  * results when few rows make it worth splitting the keys; it is the caller's for the
  * duration of the call's work on `stream`, and needs no initial contents.

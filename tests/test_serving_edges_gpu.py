@@ -6,7 +6,7 @@ import torch
 
 import cuda_ai_kernels as K
 from conftest import assert_device_clean
-from test_serving_gpu import TYPES, NAN, check_prompt, offsets, prompt_inputs
+from test_serving_gpu import TYPES, NAN, attention_bound, check_prompt, offsets, prompt_inputs, within
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +46,34 @@ def test_every_row_is_in_front_of_the_first_sequence(dtype):
         cu = torch.tensor([first], dtype=torch.int32, device="cuda")
         leave_nan_in_the_allocator(q)
         assert bool((K.attention_prompt(q, k, v, cu, cu) == 0).all())
+
+
+# ------------------------------------------------------------------------------ very many sequences
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("sequences,keys,heads", [(20000, 511, 1), (3000, 4000, 4)])
+def test_many_single_tokens_at_the_end_of_long_keys(sequences, keys, heads, dtype, abi):
+    # Units of all sequences times blocks of all keys would be more than 2^31: each sees its own only.
+    dim = 8
+    q, k, v = prompt_inputs(42, [sequences], [sequences * keys], heads, 1, dim, dtype)
+    cu_q = torch.arange(sequences + 1, dtype=torch.int32, device="cuda")
+    out = K.attention_prompt(q, k, v, cu_q, cu_q * keys)
+    scale = float(torch.tensor(dim ** -0.5, dtype=torch.float32))
+    q64, k64, v64 = q.double(), k.double().view(sequences, keys, dim), v.double().view(sequences, keys, dim)
+    p = torch.softmax(torch.bmm(q64, k64.transpose(1, 2)) * scale, dim=-1)
+    size = (torch.bmm(q64.abs(), k64.abs().transpose(1, 2)) * scale).amax(-1, keepdim=True)
+    within(out, torch.bmm(p, v64), attention_bound(torch.bmm(p, v64), torch.bmm(p, v64.abs()), size, dim, keys, dtype))
+    assert_device_clean(abi)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("q_rows,k_rows,heads,kv_heads", [(1 << 20, 1 << 20, 32, 32), (400000, 1 << 20, 96, 32)])
+def test_arrays_large_enough_for_positions_of_64_bits(q_rows, k_rows, heads, kv_heads, causal, dtype, abi):
+    # All queries over all keys would pass 32 bits; these sequences use a corner of the arrays.
+    q_lens, k_lens, dim = [300, 0, 5, 1, 1100], [700, 9, 5, 3000, 1100], 8
+    q, k, v = prompt_inputs(43, [q_rows], [k_rows], heads, kv_heads, dim, dtype)
+    out = K.attention_prompt(q, k, v, offsets(q_lens), offsets(k_lens), causal=causal)
+    check_prompt(out, q, k, v, q_lens, k_lens, causal=causal)
+    assert torch.equal(out, K.attention_prompt(q, k, v, offsets(q_lens), offsets(k_lens), causal=causal))
+    assert_device_clean(abi)
