@@ -222,14 +222,13 @@ Plan plan(AttentionArgs* a) {
     ranges = (prefix * longest + own * blocks(a->room)) * a->kv_heads;
     most = (ranges << a->pair_shift) + (prefix + own) * a->kv_heads * a->unit_cost;
   } else {
-    // Each sequence, and the rows in front of them and behind them, rounds up once. (A call has rows in
-    // front only where its first offset is not zero: they are not counted on for the grid.)
+    // Each sequence, and the rows behind them, rounds up once.
     const __int128 whole = a->q_rows / a->tokens, all = whole + a->sequences + 1;
     ranges = all * a->kv_heads * (longest > 0 ? longest : 1);
     // A sequence of n queries and m keys has at most n / tokens + 1 units of m / keys + 1 blocks. Summed
     // over sequences that do not overlap: n m to at most all queries by all keys, n and m to all of them.
     const __int128 all_keys = a->k_rows / keys + 1;
-    most = ((((whole + 1) * all_keys + whole + 1 + all_keys + a->sequences) << a->pair_shift) + (all + 1) * a->unit_cost) * a->kv_heads;
+    most = ((((whole + 1) * all_keys + whole + 1 + all_keys + a->sequences) << a->pair_shift) + all * a->unit_cost) * a->kv_heads;
   }
   // On the device the line is counted in 64 bits, with room for a sum per thread. It would take years to
   // work through.

@@ -2,8 +2,8 @@
 // partial results (attention.cu).
 //
 // Both operators are lists of sequences: n query tokens that see m keys. A prompt call has one per
-// packed sequence (and then one for the rows behind them and one for the rows in front of them, which
-// see nothing); a shared-prefix call has the whole batch over the prefix first and then every request
+// packed sequence (and a last one for the rows behind them, which sees nothing; the rows in front of
+// them are cleared apart from all that); a shared-prefix call has the whole batch over the prefix first and then every request
 // over its own part of the cache. The rows of a key head are (token, query head of its group) pairs in that order, row
 // i * group + g, so that all rows that read the same keys sit side by side whatever the head layout
 // is: a decoding batch fills a tile with requests and heads as a prompt fills it with tokens.
@@ -42,7 +42,7 @@ struct AttentionArgs {
   void* out;
   const int32_t *cu_q, *cu_k, *lengths;
   int kind, dtype;
-  int sequences;                     // prompt: without the rows in front and behind; shared: 1 + batch
+  int sequences;                     // prompt: without the rows behind the last one; shared: 1 + batch
   int q_rows, k_rows, room;          // k_rows: keys of the packed array, or of the prefix
   int heads, kv_heads, group, dim;
   float scale_log2;                  // scale * log2(e): exponentials are powers of two
@@ -85,7 +85,7 @@ inline int log2_or_minus_one(int v) {
 
 __host__ __device__ inline int clamp_int(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
 
-__device__ __forceinline__ int sequence_count(const AttentionArgs& a) { return a.sequences + (a.kind == kPrompt ? 2 : 0); }
+__device__ __forceinline__ int sequence_count(const AttentionArgs& a) { return a.sequences + (a.kind == kPrompt ? 1 : 0); }
 
 __device__ __forceinline__ Sequence sequence_of(const AttentionArgs& a, int s) {
   Sequence r{};
@@ -98,15 +98,9 @@ __device__ __forceinline__ Sequence sequence_of(const AttentionArgs& a, int s) {
     }
     return r;
   }
-  const bool front = s > a.sequences;
-  const int from = front ? 0 : s, next = min(s + 1, a.sequences);   // all four on their way at once
-  const int q0 = __ldg(a.cu_q + from), q1 = __ldg(a.cu_q + next), k0 = __ldg(a.cu_k + from), k1 = __ldg(a.cu_k + next);
-  const int first = clamp_int(q0, 0, a.q_rows);
-  if (front) {
-    r.n = first;
-    return r;
-  }
-  r.q_row = first;
+  const int next = min(s + 1, a.sequences);   // all four on their way at once
+  const int q0 = __ldg(a.cu_q + s), q1 = __ldg(a.cu_q + next), k0 = __ldg(a.cu_k + s), k1 = __ldg(a.cu_k + next);
+  r.q_row = clamp_int(q0, 0, a.q_rows);
   r.k_row = clamp_int(k0, 0, a.k_rows);
   if (s == a.sequences) {
     r.n = a.q_rows - r.q_row;
@@ -211,9 +205,11 @@ struct Ranges {
   }
 };
 
+constexpr int kIdle = -1, kRefused = -2;
+
 template <typename Line>
 struct WorkStart {
-  int sequence;               // -1: nothing to do
+  int sequence;               // kIdle: nothing to do; kRefused: in the whole call
   Sequence seq;
   int units;                  // of a head of the sequence
   int head, unit;
@@ -252,14 +248,15 @@ __device__ __forceinline__ WorkStart<Line> find_range(const AttentionArgs& a, Wo
   }
   if ((threadIdx.x & 31) == 31) scratch->sums[threadIdx.x >> 5] = upto;
   WorkStart<Line>& start = scratch->start;
-  if (threadIdx.x == 0) start.sequence = -1;
+  if (threadIdx.x == 0) start.sequence = kIdle;
   __syncthreads();
   int64_t ahead = upto - mine, whole = 0;
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < static_cast<int>(threadIdx.x >> 5)) ahead += scratch->sums[w];
     whole += scratch->sums[w];
   }
-  const Line total = whole <= a.longest_line ? static_cast<Line>(whole) : 0;   // too long: nothing is done
+  const Line total = whole <= a.longest_line ? static_cast<Line>(whole) : 0;
+  if (whole > a.longest_line && threadIdx.x == 0) start.sequence = kRefused;   // sequences overlap
   Line before = static_cast<Line>(min(ahead, static_cast<int64_t>(total)));
   const Ranges<Line> ranges(total, a.ctas);
   const Line begin = ranges.begin(blockIdx.x), length = ranges.begin(blockIdx.x + 1) - begin;
@@ -296,6 +293,17 @@ __device__ __forceinline__ WorkStart<Line> find_range(const AttentionArgs& a, Wo
     low = start.unit, high = min(low + step, high);
     if (step <= 1) return start;
   }
+}
+
+// Zeros for the rows that no sequence owns: those in front of the first one, or all of a call whose
+// sequences overlap so far that their work has no bound, which is recorded. By some threads of every CTA.
+static __device__ __noinline__ void clear_unowned_rows(const AttentionArgs& a, bool refused, int thread, int threads) {
+  if (a.kind != kPrompt) return;
+  const int64_t rows = refused ? a.q_rows : clamp_int(__ldg(a.cu_q), 0, a.q_rows);
+  const int64_t granules = rows * a.heads * a.dim / (a.dtype == B200_FP32 ? 4 : 8);
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * threads + thread; i < granules; i += static_cast<int64_t>(gridDim.x) * threads)
+    static_cast<uint4*>(a.out)[i] = make_uint4(0, 0, 0, 0);
+  if (refused && blockIdx.x == 0 && thread == 0) atomicOr(&g_device_status, kSiteOverlap);
 }
 
 // A contiguous run of key blocks of one unit.

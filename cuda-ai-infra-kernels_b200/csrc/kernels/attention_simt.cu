@@ -16,6 +16,9 @@
 #include "attention.cuh"
 
 namespace b200 {
+
+cudaError_t attention_simt_status_read_clear(uint32_t* word) { return status_word_read_clear(word); }
+
 namespace {
 
 constexpr int kKeys = kSimtKeyBlock;
@@ -73,7 +76,9 @@ __global__ void __launch_bounds__(kThreads, kRows == 16 ? 4 : kRows == 64 ? 2 : 
   grid_launch_dependents();
   grid_dependency_wait();
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  SegmentWalk<kKeys, Line> walk(a, find_range<kKeys, kThreads, Line>(a, &scratch));
+  const WorkStart<Line> start = find_range<kKeys, kThreads, Line>(a, &scratch);
+  clear_unowned_rows(a, start.sequence == kRefused, threadIdx.x, kThreads);
+  SegmentWalk<kKeys, Line> walk(a, start);
   Segment g;
   if (threadIdx.x == 0) start_records(a);
   while (walk.next(&g)) {

@@ -201,6 +201,7 @@ __device__ __forceinline__ void segment_role(const UmmaAttentionArgs& p, const W
     clear(count % kDelay);   // the segment before the last one
     if (!more) {
       clear((count + 1) % kDelay);
+      clear_unowned_rows(a, start.sequence == kRefused, lane, 32);   // last: nobody waits for it
       return;
     }
     if (e.blocks > 0) {

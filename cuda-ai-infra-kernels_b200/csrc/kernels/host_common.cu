@@ -189,9 +189,11 @@ int b200_device_status_read(uint32_t* host_word, b200_stream_t stream) {
   if (b200::peer_sync_status_read_clear(&peer_word) != cudaSuccess) return B200_ERR_LAUNCH_FAILED;
   uint32_t row_word = 0;
   if (b200::rowops_status_read_clear(&row_word) != cudaSuccess) return B200_ERR_LAUNCH_FAILED;
-  uint32_t attention_word = 0;
+  uint32_t attention_word = 0, attention_simt_word = 0;
   if (b200::attention_status_read_clear(&attention_word) != cudaSuccess) return B200_ERR_LAUNCH_FAILED;
-  *host_word = sgemm_word | umma_word | selftest_word | peer_word | row_word | attention_word;
+  if (b200::attention_simt_status_read_clear(&attention_simt_word) != cudaSuccess) return B200_ERR_LAUNCH_FAILED;
+  *host_word = sgemm_word | umma_word | selftest_word | peer_word | row_word | attention_word | attention_simt_word;
+  if (*host_word == B200_ATTENTION_OVERLAP) return B200_ERR_INVALID_ARGUMENT;
   return *host_word == 0 ? B200_OK : B200_ERR_DEVICE_TIMEOUT;
 }
 

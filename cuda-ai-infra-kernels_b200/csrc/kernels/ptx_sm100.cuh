@@ -41,6 +41,7 @@ enum WaitSite : uint32_t {
   kSiteRowStaged = 1u << 9,   // row operators: the staged row never arrived
   kSiteBounds = 1u << 10,   // debug build only: an index check failed and the access was skipped
   kSiteAttention = 1u << 11,   // attention: a pipeline stage never arrived
+  kSiteOverlap = 1u << 12,   // no wait: attention refused sequences that overlap
 };
 
 // Debug build (-DB200_DEBUG_BOUNDS, a separate library; never the shipped one): the stores and the

@@ -72,7 +72,8 @@ const char* b200_build_info(void);
 int b200_device_status_read(uint32_t* host_word, b200_stream_t stream);
 
 /*
- * Bits of the status word: which wait gave up.
+ * Bits of the status word: which wait gave up (B200_ERR_DEVICE_TIMEOUT), or, as the only one that
+ * is none (B200_ERR_INVALID_ARGUMENT where it stands alone), offsets that were refused on the device.
  */
 enum {
   B200_WAIT_SGEMM_FULL = 1 << 0,    /* FP32 pipeline: consumer waiting for a TMA stage */
@@ -85,7 +86,8 @@ enum {
   B200_WAIT_SELFTEST = 1 << 7,      /* b200_selftest_wait_gives_up */
   B200_WAIT_PEER_BARRIER = 1 << 8,  /* b200_peer_barrier: a peer never signalled the step */
   B200_WAIT_ROW_STAGED = 1 << 9,    /* row operators: a row staged by the copy engine never arrived */
-  B200_WAIT_ATTENTION = 1 << 11     /* attention: a pipeline stage never arrived (bit 10: debug build's index checks) */
+  B200_WAIT_ATTENTION = 1 << 11,    /* attention: a pipeline stage never arrived (bit 10: debug build's index checks) */
+  B200_ATTENTION_OVERLAP = 1 << 12  /* b200_attention_prompt: sequences overlap; the output is zero */
 };
 
 /*
@@ -368,6 +370,10 @@ typedef struct b200_rows_view {
  *   (B200_ERR_MISALIGNED_OPERAND otherwise); out is dense [tokens][heads][dim].
  * cu_q and cu_k are device arrays of sequences + 1 offsets; they are read by the
  * kernels only, and offsets outside the arrays do not lead to accesses outside them.
+ * Offsets that fall, so that sequences overlap, are the caller's mistake: where their work
+ * is more than any sequences that do not overlap could make of the arrays, the output is
+ * zero and the status word gets B200_ATTENTION_OVERLAP; else rows that several sequences
+ * own hold a mixture of their results.
  * B200_ERR_INVALID_PROBLEM: rows, or query rows times heads / kv_heads, above 2^30.
  * `workspace` (16-byte aligned, b200_attention_prompt_workspace_bytes) holds partial
  * results when few rows make it worth splitting the keys; it is the caller's for the

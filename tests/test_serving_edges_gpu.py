@@ -1,11 +1,13 @@
 """The serving operators where their callers come to the edges of what is documented: rows in front of the
 first sequence, offsets that overlap, probabilities far below a row's largest, gradients of either mode.
 Helpers and the derivation of the tolerances: test_serving_gpu.py."""
+import ctypes
+
 import pytest
 import torch
 
 import cuda_ai_kernels as K
-from conftest import assert_device_clean
+from conftest import assert_device_clean, current_stream_ptr
 from test_serving_gpu import TYPES, NAN, attention_bound, check_prompt, offsets, prompt_inputs, within
 
 pytestmark = pytest.mark.gpu
@@ -76,4 +78,31 @@ def test_arrays_large_enough_for_positions_of_64_bits(q_rows, k_rows, heads, kv_
     out = K.attention_prompt(q, k, v, offsets(q_lens), offsets(k_lens), causal=causal)
     check_prompt(out, q, k, v, q_lens, k_lens, causal=causal)
     assert torch.equal(out, K.attention_prompt(q, k, v, offsets(q_lens), offsets(k_lens), causal=causal))
+    assert_device_clean(abi)
+
+
+# ------------------------------------------------------------------------------- overlapping offsets
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_offsets_that_overlap_too_much_give_zeros_and_a_status(dtype, abi):
+    # Twenty sequences that all claim all rows, with falling offsets between them.
+    rows = 4096
+    q, k, v = prompt_inputs(44, [rows], [rows], 4, 2, 64, dtype)
+    cu = torch.tensor([0, rows] * 20, dtype=torch.int32, device="cuda")
+    assert_device_clean(abi)
+    leave_nan_in_the_allocator(q)
+    out = K.attention_prompt(q, k, v, cu)
+    word = ctypes.c_uint32(0)
+    assert abi.b200_device_status_read(ctypes.byref(word), ctypes.c_void_p(current_stream_ptr())) == 4   # invalid argument
+    assert word.value == 1 << 12
+    assert bool((out == 0).all())
+    check_prompt(K.attention_prompt(q, k, v, offsets([rows])), q, k, v, [rows], [rows])
+    assert_device_clean(abi)
+
+
+def test_falling_offsets_still_define_every_row(abi):
+    q, k, v = prompt_inputs(45, [64], [64], 4, 2, 64, torch.bfloat16)
+    for bad in ([0, 1000], [-50, 64], [0, 40, 20, 64], [70, 90], [50, 20], [30, 10, 64, 0]):
+        leave_nan_in_the_allocator(q)
+        assert bool(torch.isfinite(K.attention_prompt(q, k, v, torch.tensor(bad, dtype=torch.int32, device="cuda"))).all())
     assert_device_clean(abi)
