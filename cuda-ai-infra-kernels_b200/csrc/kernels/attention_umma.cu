@@ -5,7 +5,9 @@
 // tensor memory as a 16-bit operand in columns that held S, and O += P V with P read from there. O
 // stays in tensor memory for the whole unit. P is rounded to the operand type (at most 2^-8 or 2^-11
 // of a probability, as the output's own rounding); the denominator adds up the unrounded
-// FP32 values.
+// FP32 values. FP16 holds P times 2^7, which it has the room for: unscaled, a probability below 2^-14 of
+// the largest would be subnormal and one below 2^-25 nothing, and 100000 such keys are 0.003 of the row.
+// So the limits are 2^-21 and 2^-32, and what is lost below them is at most 2^-32 per key.
 //
 // Two streams, each with its own group of four warps, O and S: the two row tiles of a unit of 256
 // rows, over the same blocks of 128 keys; or, where a unit has at most one tile of rows (a decoding
@@ -20,7 +22,7 @@
 //
 // The maximum is followed lazily: O and the denominator are rescaled only when a row's maximum has
 // grown by more than 2^8 since the last time, which the first block or two settle. Until then
-// P <= 256 and nothing overflows; the quotient is the same.
+// P <= 2^8 (FP16: 2^15) and nothing overflows; the quotient is the same.
 //
 // Warps 0-3 and 4-7: streams 0 and 1, warp w owning TMEM lanes 32 (w mod 4) ... Warp 8: copies (TMA).
 // Warps 9 and 10: one MMA-issuing thread per stream (a lone thread spends as long on barriers and
@@ -43,6 +45,7 @@ static_assert(256 * kSoftmaxRegisters + 128 * kOtherRegisters <= kThreads * 168,
 constexpr int kTile = 128;          // rows of a tile, keys of a block
 constexpr float kMinusInf = -__builtin_huge_valf();
 constexpr float kLazy = 8.f;        // growth of a maximum, in powers of two, that forces a rescale
+constexpr float kRaiseFp16 = 7.f;   // FP16 holds P times 2^7
 constexpr int kHalf = 64;           // keys of one S
 constexpr uint32_t kColS = 0, kColO = 256, kColStream = 128, kColHalf = 64;   // TMEM columns
 
@@ -390,6 +393,7 @@ __device__ __forceinline__ void softmax_half(uint32_t s_at, uint32_t o_at, int c
   float m = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]) * scale;
   if (m == -kMinusInf) m = __int_as_float(0x7fffffff);
   if (!live) m = 0.f;   // lanes without a row hold anything; they must not ask for rescaling
+  if (!kBf16) m -= kRaiseFp16;
   if (first) {
     row->m = m;
   } else {

@@ -2,6 +2,7 @@
 first sequence, offsets that overlap, probabilities far below a row's largest, gradients of either mode.
 Helpers and the derivation of the tolerances: test_serving_gpu.py."""
 import ctypes
+import math
 
 import pytest
 import torch
@@ -106,3 +107,56 @@ def test_falling_offsets_still_define_every_row(abi):
         leave_nan_in_the_allocator(q)
         assert bool(torch.isfinite(K.attention_prompt(q, k, v, torch.tensor(bad, dtype=torch.int32, device="cuda"))).all())
     assert_device_clean(abi)
+
+
+# ------------------------------------------------------- probabilities far below a row's largest
+
+def sink(rows, keys, gap, dtype, place, dim=64):
+    """One key whose score is `gap` above all others', and its value zero where theirs are one."""
+    q, k = torch.zeros(rows, 2, dim, device="cuda"), torch.zeros(keys, 2, dim, device="cuda")
+    q[..., 0], k[place, :, 0] = 1.0, gap
+    v = torch.ones(keys, 2, dim, device="cuda")
+    v[place] = 0.0
+    return q.to(dtype), k.to(dtype), v.to(dtype)
+
+
+def check_sink(out, keys, gap, dtype):
+    # Others weigh w = (keys - 1) 2^(-gap log2 e) against one. What test_serving_gpu.py derives holds while a
+    # probability rounds relative to itself. FP16 holds it times 2^7 (at most 2^15), so that below 2^-21 of the
+    # largest it rounds to multiples of 2^-24 instead: half of that, 2^-32 of the largest, for each key.
+    w = (keys - 1) * math.exp(-gap)
+    expected = torch.full(out.shape, w / (1 + w), dtype=torch.float64, device="cuda")
+    far = keys * 2.0 ** -32 if dtype == torch.float16 else 0.0
+    within(out, expected, attention_bound(expected, expected, torch.full_like(expected[..., :1], gap), out.shape[-1], keys, dtype) + far)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("gap", [17.546875, 16.5, 12.0, 19.0])   # 2^-25.3, 2^-23.8, 2^-17.3, 2^-27.4; exact in the types but BF16's 17.5
+@pytest.mark.parametrize("keys", [32768, 131072])
+@pytest.mark.parametrize("place", [0, -1, 5000])
+def test_many_keys_far_below_the_largest_still_count(keys, gap, place, dtype):
+    gap = float(torch.tensor(gap, dtype=dtype))
+    # One row, whose keys are dealt out over all CTAs, and so many that a CTA meets all keys of its rows.
+    rows = 20000
+    q, k, v = sink(rows, keys, gap, dtype, place)
+    check_sink(K.attention_prompt(q[:1], k, v, offsets([1]), offsets([keys]), scale=1.0), keys, gap, dtype)
+    check_sink(K.attention_prompt(q, k, v, offsets([rows]), offsets([keys]), causal=False, scale=1.0), keys, gap, dtype)
+    # The same keys as a prefix and a request's own part.
+    own = 16
+    cut = keys - own
+    cache = [t[cut:].expand(rows, own, 2, 64).contiguous() for t in (k, v)]
+    lengths = torch.full((rows,), own, dtype=torch.int32, device="cuda")
+    check_sink(K.attention_shared_prefix(q, k[:cut], v[:cut], *cache, lengths, scale=1.0), keys, gap, dtype)
+
+
+def test_fp16_probabilities_stay_in_range_while_the_maximum_grows():
+    # The maximum is followed lazily: a row's scores may be 2^8 above the base of its exponentials.
+    keys = 640
+    steps = torch.arange(keys, device="cuda") // 64                        # a block of scores after the other,
+    for each in (5.0, 5.5, 5.6, 2.75):                                     # 2^7.2, 2^7.9, 2^8.1 and 2^4 apart
+        q, k = torch.zeros(300, 2, 64, device="cuda").half(), torch.zeros(keys, 2, 64, device="cuda").half()
+        q[..., 0] = 1.0
+        k[:, :, 0] = (steps * each).half()[:, None]
+        v = torch.full((keys, 2, 64), 60000.0, device="cuda").half()
+        out = K.attention_prompt(q, k, v, offsets([300]), offsets([keys]), causal=False, scale=1.0)
+        check_prompt(out, q, k, v, [300], [keys], scale=1.0, causal=False)
