@@ -1,6 +1,8 @@
 // PyTorch-facing launchers of the serving operators: attention over packed prompts and over a shared
 // prefix, the 4-bit matrix-vector product, and the processing of logits. The reference has none of
 // them; argument rules and message style are those of the other launchers here.
+#include <c10/core/AutogradState.h>
+
 #include <cmath>
 
 #include "op_common.h"
@@ -20,10 +22,13 @@ int dtype_of(const torch::Tensor& t, const char* name) {
   }
 }
 
-// These operators compute no gradient: a graph that would need one is refused instead of being cut.
+// These operators compute no gradient: a graph that would need one, backward or forward, is refused
+// instead of being cut. (torch.no_grad() does not switch tangents off.)
 void check_no_gradient(const torch::Tensor& t, const char* name) {
   TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), name,
               " requires a gradient, which this operator does not compute; call it under torch.no_grad()");
+  TORCH_CHECK(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined()), name,
+              " carries a forward-mode tangent, which this operator does not propagate; pass its primal");
 }
 
 void check_same(const torch::Tensor& t, const char* name, const torch::Tensor& first, const char* first_name) {

@@ -119,7 +119,7 @@ def adaptive_gemm(
 # ---------------------------------------------------------------- serving operators
 # What one serving step of a decoder needs next to the products and row operators above. The
 # reference has none of them. They compute no gradient (inputs that require one are refused outside
-# ``torch.no_grad()``), run on the inputs' device and its current stream, read lengths and offsets on
+# ``torch.no_grad()``, inputs with a forward-mode tangent always), run on the inputs' device and its current stream, read lengths and offsets on
 # the device only, and may be captured in CUDA graphs.
 
 

@@ -9,7 +9,8 @@ import torch
 
 import cuda_ai_kernels as K
 from conftest import assert_device_clean, current_stream_ptr
-from test_serving_gpu import TYPES, NAN, attention_bound, check_prompt, offsets, prompt_inputs, within
+from test_serving_gpu import (TYPES, NAN, attention_bound, check_prompt, logits_inputs, offsets, prompt_inputs, shared_inputs,
+                              w4_inputs, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -160,3 +161,32 @@ def test_fp16_probabilities_stay_in_range_while_the_maximum_grows():
         v = torch.full((keys, 2, 64), 60000.0, device="cuda").half()
         out = K.attention_prompt(q, k, v, offsets([300]), offsets([keys]), causal=False, scale=1.0)
         check_prompt(out, q, k, v, [300], [keys], scale=1.0, causal=False)
+
+
+# ------------------------------------------------------------------------------ forward-mode tangents
+
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as forward
+
+    half = torch.float16
+    q, k, v = prompt_inputs(46, [5], [5], 4, 2, 64, half)
+    shared = shared_inputs(47, 2, 10, 4, 4, 2, 64, half)
+    lengths, cu = torch.ones(2, dtype=torch.int32, device="cuda"), offsets([5])
+    x, qweight, scales, _ = w4_inputs(48, 2, 8, 128, 64, half, False)
+    logits = logits_inputs(49, 2, 100, 5, 5, 2, half)
+    with forward.dual_level():
+        dual = lambda t: forward.make_dual(t, torch.ones_like(t))  # noqa: E731
+        calls = [lambda i=i: K.attention_prompt(*[dual(t) if j == i else t for j, t in enumerate((q, k, v))], cu) for i in range(3)]
+        calls += [lambda i=i: K.attention_shared_prefix(*[dual(t) if j == i else t for j, t in enumerate(shared)], lengths) for i in range(5)]
+        calls += [lambda: K.matvec_w4(dual(x), qweight, scales), lambda: K.matvec_w4(x, qweight, dual(scales))]
+        calls += [lambda n=n: K.process_logits(**{**logits, n: dual(logits[n])})
+                  for n in ("logits", "repetition_penalty", "frequency_penalty", "presence_penalty", "bias_values")]
+        for call in calls:
+            with pytest.raises(RuntimeError, match="forward-mode tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode tangent"):
+                call()
+        expected = K.attention_prompt(q, k, v, cu)
+        assert torch.equal(K.attention_prompt(forward.unpack_dual(dual(q)).primal, k, v, cu), expected)
+        with forward._set_fwd_grad_enabled(False):
+            assert torch.equal(K.attention_prompt(dual(q), k, v, cu), expected)
