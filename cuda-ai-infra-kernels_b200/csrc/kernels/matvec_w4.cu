@@ -138,12 +138,13 @@ __device__ __forceinline__ void load_pairs(uint32_t (&out)[4], const T* p, int) 
   out[0] = __byte_perm(v.x, v.z, 0x5410), out[1] = __byte_perm(v.x, v.z, 0x7632);
   out[2] = __byte_perm(v.y, v.w, 0x5410), out[3] = __byte_perm(v.y, v.w, 0x7632);
 }
-// Term `part` of a finite FP32 number as a sum of three BF16 ones, in the upper half of the result.
+// Term `part` of an FP32 number as a sum of three BF16 ones, in the upper half of the result.
 __device__ __forceinline__ uint32_t bf16_term(float x, int part) {
   const uint32_t hi = __float_as_uint(x) & 0xffff0000u;
   if (part == 0) return hi;
-  // What an infinity or a NaN leaves is nothing: the first term carries it alone.
-  const float r1 = (hi & 0x7f800000u) == 0x7f800000u ? 0.f : x - __uint_as_float(hi);
+  // What an infinity leaves is nothing: the first term carries it alone. What a NaN leaves is one, so that
+  // it stays one even where its first term reads as an infinity (a payload in the lower half only).
+  const float r1 = fabsf(x) == __uint_as_float(0x7f800000u) ? 0.f : x - __uint_as_float(hi);
   const uint32_t mid = __float_as_uint(r1) & 0xffff0000u;
   if (part == 1) return mid;
   return __float_as_uint(r1 - __uint_as_float(mid));

@@ -190,3 +190,16 @@ def test_forward_mode_tangents_are_refused():
         assert torch.equal(K.attention_prompt(forward.unpack_dual(dual(q)).primal, k, v, cu), expected)
         with forward._set_fwd_grad_enabled(False):
             assert torch.equal(K.attention_prompt(dual(q), k, v, cu), expected)
+
+
+# ------------------------------------------------------------------------------- FP32 4-bit product
+
+@pytest.mark.parametrize("bits", [0x7f800001, 0x7f80ffff, 0x7fbf0000, 0x7fc00000, 0xff800001 - (1 << 32), 0xffc00000 - (1 << 32)], ids=hex)
+@pytest.mark.parametrize("rows", [1, 4, 16])
+def test_matvec_w4_every_nan_stays_one(rows, bits):
+    x, qweight, scales, _ = w4_inputs(50, rows, 40, 256, 64, torch.float32, False)
+    qweight[:] = 0x99   # all weights one step above zero
+    clean = K.matvec_w4(x, qweight, scales)
+    x.view(torch.int32)[rows - 1, 77] = bits
+    out = K.matvec_w4(x, qweight, scales)
+    assert bool(torch.isnan(out[rows - 1]).all()) and torch.equal(out[:rows - 1], clean[:rows - 1])
