@@ -286,8 +286,7 @@ template <typename T, int kTiles, int kBytes>
 int launch(const b200_matvec_w4_problem& q, cudaStream_t s) {
   constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
   if constexpr (kTiles <= 3 && kBytes >= (kParts == 3 ? 8 : 16)) {
-    constexpr int kLarge = 2 * 148 * 32;
-    if (q.rows * kParts >= 6 && q.n >= kLarge) return launch_shape<T, kTiles, kBytes, 2, 8>(q, s);
+    if (q.rows * kParts >= 6 && q.n >= 2 * 32 * sm_count()) return launch_shape<T, kTiles, kBytes, 2, 8>(q, s);
   }
   // Few CTAs: as many warps in each as leave all CTAs room at once, one or two per multiprocessor. 16
   // against 8 warps, BF16: one row by 4096 x 4096 5.7 and 8.3 us, by 4096 x 14336 12.1 and 22.6, 16 rows
@@ -296,10 +295,10 @@ int launch(const b200_matvec_w4_problem& q, cudaStream_t s) {
   // More CTAs than that lose by it (16 rows by 5120 x 5120 13.5 with 8 warps, 18.9 with 12).
   if constexpr (kTiles <= 3) {
     constexpr bool kSmall = kTiles == 1 && kParts == 1;
-    constexpr int kRound = 148 * 16;   // rows of one CTA per multiprocessor
-    if (q.n <= (kSmall ? 2 * kRound : kRound)) return launch_shape<T, kTiles, kBytes, 1, 16>(q, s);
+    const int round = 16 * sm_count();   // rows of one CTA per multiprocessor
+    if (q.n <= (kSmall ? 2 * round : round)) return launch_shape<T, kTiles, kBytes, 1, 16>(q, s);
     if constexpr (!kSmall) {
-      if (q.n <= 2 * kRound) return launch_shape<T, kTiles, kBytes, 1, 12>(q, s);
+      if (q.n <= 2 * round) return launch_shape<T, kTiles, kBytes, 1, 12>(q, s);
     }
   }
   return launch_shape<T, kTiles, kBytes, 1, 8>(q, s);

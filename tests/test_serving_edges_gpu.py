@@ -9,7 +9,7 @@ import torch
 
 import cuda_ai_kernels as K
 from conftest import assert_device_clean, current_stream_ptr
-from test_serving_gpu import (TYPES, NAN, attention_bound, check_prompt, logits_inputs, offsets, prompt_inputs, shared_inputs,
+from test_serving_gpu import (TYPES, NAN, attention_bound, check_prompt, check_w4, logits_inputs, offsets, prompt_inputs, shared_inputs,
                               w4_inputs, within)
 
 pytestmark = pytest.mark.gpu
@@ -203,3 +203,14 @@ def test_matvec_w4_every_nan_stays_one(rows, bits):
     x.view(torch.int32)[rows - 1, 77] = bits
     out = K.matvec_w4(x, qweight, scales)
     assert bool(torch.isnan(out[rows - 1]).all()) and torch.equal(out[:rows - 1], clean[:rows - 1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 6, 9, 16])
+@pytest.mark.parametrize("ctas,height", [(1, 16), (2, 16), (2, 32)])
+def test_matvec_w4_around_the_sizes_at_which_a_cta_changes(ctas, height, rows, dtype):
+    # Rows of weights that make one or two CTAs per multiprocessor of this machine, one less and one more.
+    here = ctas * height * torch.cuda.get_device_properties(0).multi_processor_count
+    for n in (here - 1, here, here + 1):
+        x, qweight, scales, z = w4_inputs(51, rows, n, 256, 128, dtype, True)
+        check_w4(K.matvec_w4(x, qweight, scales, z), x, qweight, scales, z)
