@@ -43,10 +43,15 @@ void check_array(const torch::Tensor& t, const char* name, int64_t dims, const t
   check_no_gradient(t, name);
 }
 
+void check_limit(int64_t rows, const char* name, const char* what = "rows") {
+  TORCH_CHECK(rows <= int64_t{1} << 30, name, " has too many ", what);
+}
+
 torch::Tensor int32_vector(const torch::Tensor& t, const char* name, const torch::Tensor& first, const char* first_name) {
   check_same(t, name, first, first_name);
   TORCH_CHECK(t.scalar_type() == torch::kInt32, name, " must be int32");
   TORCH_CHECK(t.dim() == 1, name, " must be 1-dimensional");
+  check_limit(t.size(0) - 1, name, "entries");   // sequences and requests are counted in 32 bits
   return t.contiguous();
 }
 
@@ -75,12 +80,9 @@ float scale_or_default(const c10::optional<double>& scale, int64_t dim) {
 void check_heads(const torch::Tensor& q, int64_t kv_heads) {
   const int64_t heads = q.size(1), dim = q.size(2);
   TORCH_CHECK(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "the number of query heads must be a multiple of the number of key heads");
+  check_limit(heads, "q", "heads");
   TORCH_CHECK(heads / kv_heads <= 128, "at most 128 query heads per key head are supported");
   TORCH_CHECK(dim > 0 && dim % 8 == 0 && dim <= 128, "head dimension must be a multiple of 8 up to 128");
-}
-
-void check_limit(int64_t rows, const char* name) {
-  TORCH_CHECK(rows <= int64_t{1} << 30, name, " has too many rows");
 }
 
 }  // namespace

@@ -214,3 +214,18 @@ def test_matvec_w4_around_the_sizes_at_which_a_cta_changes(ctas, height, rows, d
     for n in (here - 1, here, here + 1):
         x, qweight, scales, z = w4_inputs(51, rows, n, 256, 128, dtype, True)
         check_w4(K.matvec_w4(x, qweight, scales, z), x, qweight, scales, z)
+
+
+# ------------------------------------------------------------------------- counts that pass 32 bits
+
+def test_more_sequences_or_heads_than_32_bits_count_are_refused():
+    q, k, v = prompt_inputs(52, [5], [5], 1, 1, 64, torch.float16)
+    many = torch.zeros(1, dtype=torch.int32, device="cuda").expand(2 ** 32 + 2)   # would read as one sequence
+    with pytest.raises(RuntimeError, match="too many entries"):
+        K.attention_prompt(q, k, v, many)
+    with pytest.raises(RuntimeError, match="too many entries"):
+        K.attention_prompt(q, k, v, offsets([5]), many)
+    none, heads = q[:0], 2 ** 32 + 1                                              # would read as one head
+    with pytest.raises(RuntimeError, match="too many heads"):
+        K.attention_prompt(*[t[:0].expand(0, heads, 64) for t in (q, k, v)], offsets([]))
+    assert K.attention_prompt(none, none, none, offsets([])).shape == none.shape
