@@ -115,7 +115,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_rows_kernel(co
   join.store(static_cast<int64_t>(request) * a.heads + head * a.group + g);
 }
 
-// FP32 operands would lose half their bits on the tensor cores; 16-bit ones lose nothing.
+// 16-bit operands lose nothing on the tensor cores. One TF32 or BF16 term of an FP32 operand holds half of
+// its bits; it would take a sum of terms, and several products for one.
 bool on_tensor_cores(const AttentionArgs& a) { return a.dtype != B200_FP32; }
 
 template <typename Kernel>

@@ -14,8 +14,9 @@
 // subtracting 1024 + zero or 128 + zero leaves c - zero, exact. Each step of K lies inside one group:
 // its FP32 product is multiplied by the group's scale when it is added to the running sum.
 //
-// What it measured: one BF16 row by 28672 x 8192 (117 MB of weights) 36.8 us, FP16 35.0, against 18.5 for
-// the weights at the copy bandwidth: issue slots 52 % busy, the integer pipe 58 %; 16 rows 71. What brought it there
+// What it measured: one BF16 row by 28672 x 8192 (117 MB of weights) 36.7 us, FP16 34.8, FP32 113, against
+// 18.5 for the weights at the copy bandwidth: the integer pipe 67 % busy, issue slots 60 %; 16 BF16 rows 73,
+// 8 FP32 rows 397. What brought it there
 // from 44.7: a code's mask and its base in one instruction (38.5), and the divisions that place a warp in
 // its row done by the host, the zero point of symmetric weights made once (36.8). What did not help, all
 // timed side by side: 32 rows per warp (x shared, half the warps: 51.5 against 44.8); more warps by fewer

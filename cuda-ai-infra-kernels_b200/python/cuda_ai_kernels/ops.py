@@ -142,7 +142,9 @@ def attention_prompt(
     of its cached keys), else all. ``scale`` defaults to ``dim ** -0.5``.
 
     Rows that see no key, and rows in front of the first sequence or behind the last, are
-    zero. Types: float32 (FP32 arithmetic), float16, bfloat16 (tensor cores, FP32 sums).
+    zero. Types: float32 (FP32 arithmetic), float16, bfloat16 (tensor cores: probabilities
+    are rounded to the type before they meet ``v``, which about doubles the variance of the
+    result's own rounding; maxima and sums are FP32).
     ``dim`` is a multiple of 8 up to 128. Strided views are taken as they are where their
     rows sit on 16-byte granules, and copied otherwise. Keys and values outside a sequence
     may hold anything; inside one, ``v`` must be finite.
@@ -162,8 +164,8 @@ def attention_shared_prefix(
     """One decoding step of a batch whose requests share a prefix.
 
     ``q`` is ``[batch, heads, dim]``, one token per request. Request ``b`` sees all of
-    ``k_prefix`` / ``v_prefix`` ``[prefix, kv_heads, dim]``, which are read once for the
-    whole batch, and the first ``lengths[b]`` rows of ``k_cache[b]`` / ``v_cache[b]``
+    ``k_prefix`` / ``v_prefix`` ``[prefix, kv_heads, dim]``, which are read once for up to
+    256 rows (request, query head of a key head; 16 to 128 in float32), and the first ``lengths[b]`` rows of ``k_cache[b]`` / ``v_cache[b]``
     (``[batch, room, kv_heads, dim]``); the rows behind may hold anything. Types, head
     dimensions, strides and ``scale`` as for :func:`attention_prompt`. A request that
     sees no key gets zeros.

@@ -360,12 +360,13 @@ typedef struct b200_rows_view {
  * key head h / (heads / kv_heads). With n queries and m keys, and `causal` set,
  * query i sees the keys j <= i + m - n (the last query sees all of them):
  *   out_i = sum_j p_ij v_j,  p_i = softmax over the visible j of scale * q_i . k_j.
- * A row that sees no key is zero; so are the rows in front of cu_q[0] and behind
- * cu_q[sequences]. What lies in keys or values outside a sequence is never read into
+ * A row that sees no key, or whose scores are all minus infinity, is zero; so are the
+ * rows in front of cu_q[0] and behind cu_q[sequences]. What lies in keys or values outside a sequence is never read into
  * its result, NaN and infinities included. Inside a sequence, V must be finite.
  *   dim: a multiple of 8, 8 .. 128; heads / kv_heads <= 128; scale > 0.
  *   FP16 / BF16 run on the tensor cores (probabilities rounded to the operand type
- *   for the second product, all sums in FP32); FP32 runs on the FMA pipe.
+ *   for the second product, all sums in FP32; FP16 loses at most 2^-32 of a row's
+ *   largest for each key below 2^-21 of it); FP32 runs on the FMA pipe.
  *   Pointers 16-byte aligned, strides a multiple of 16 bytes
  *   (B200_ERR_MISALIGNED_OPERAND otherwise); out is dense [tokens][heads][dim].
  * cu_q and cu_k are device arrays of sequences + 1 offsets; they are read by the
@@ -399,8 +400,9 @@ int b200_attention_prompt(const b200_attention_prompt_problem* problem, void* wo
  * One decoding step of a batch whose requests share their first `prefix` keys.
  * Request b has one query row and sees the prefix and the first lengths[b]
  * (clamped to 0 .. room) rows of its own part of the cache,
- * k_cache[b * cache_batch_stride + row * row_stride + head * head_stride + d].
- * The prefix is read once for all requests. Cache rows behind lengths[b] may hold
+ * k_cache[b * k_batch_stride + row * row_stride + head * head_stride + d].
+ * The prefix is read once per tile of rows, a row being a request and a query head of
+ * the key head: up to 256 rows in FP16 and BF16, 16 to 128 in FP32. Cache rows behind lengths[b] may hold
  * anything. Types, limits, alignment and workspace as above; a request that sees no
  * key gets zeros.
  */
