@@ -3,10 +3,11 @@
 //
 // Both operators are lists of sequences: n query tokens that see m keys. A prompt call has one per
 // packed sequence (and a last one for the rows behind them, which sees nothing; the rows in front of
-// them are cleared apart from all that); a shared-prefix call has the whole batch over the prefix first and then every request
-// over its own part of the cache. The rows of a key head are (token, query head of its group) pairs in that order, row
-// i * group + g, so that all rows that read the same keys sit side by side whatever the head layout
-// is: a decoding batch fills a tile with requests and heads as a prompt fills it with tokens.
+// them are cleared apart from all that); a shared-prefix call has the whole batch over the prefix
+// first and then every request over its own part of the cache. The rows of a key head are (token, query
+// head of its group) pairs in that order, row i * group + g, so that all rows that read the same keys
+// sit side by side whatever the head layout is: a decoding batch fills a tile with requests and heads
+// as a prompt fills it with tokens.
 //
 // A unit is `unit_rows` such rows of one key head; its keys are cut in blocks, 128 or 64 keys each. All
 // units, in the order sequence, head, unit, are laid end to end, each as long as its blocks (twice,
@@ -52,7 +53,7 @@ struct AttentionArgs {
   int token_shift;                   // its logarithm where it is a power of two, else -1
   int unit_cost, pair_shift;         // on the line: of a unit; logarithm of a block's for a unit of more than half the rows
   int ctas;                          // ranges
-  int64_t longest_line;              // that sequences which do not overlap can make
+  int64_t longest_line;              // the longest that sequences which do not overlap can make
   // Partial results, in slots of some rows: maximum (scaled, base 2) and denominator [row], and the sum,
   // not divided by it, as [dim / 4][row][4], so that the threads of a warp, which own one row
   // each, write and read whole lines. First the slots of units continued from the CTA before,
@@ -156,8 +157,8 @@ static __device__ __noinline__ int64_t floor_sum(int n, int m, int a, int b) {
   return sum;
 }
 
-// Length of the first `units` of the `all` units of one key head of the sequence. Not inlined: a CTA calls it three or four times as it starts,
-// when every instruction has to be fetched before it runs.
+// Length of the first `units` of the `all` units of one key head of the sequence. Not inlined: a CTA
+// calls it three or four times as it starts, when every instruction has to be fetched before it runs.
 template <int kKeys, typename Line>
 __device__ __noinline__ Line length_before(const AttentionArgs& a, const Sequence& s, int units, int all) {
   if (units == 0) return 0;
