@@ -16,6 +16,7 @@ drives the kernels directly partitions exactly like this module does.
 from __future__ import annotations
 
 import ctypes
+import warnings
 from pathlib import Path
 from typing import Callable, Optional, Sequence
 
@@ -135,6 +136,7 @@ def peer_row_pointers(base_ptrs: Sequence[int], rank: int, first_row: int, n: in
 
 
 WAIT_PEER_BARRIER = 1 << 8   # bit of the device status word set by a barrier that gave up
+ATTENTION_OVERLAP = 1 << 12   # no wait: attention_prompt refused offsets that overlap
 
 
 def all_ranks_ok(ok: bool, group=None) -> bool:
@@ -219,7 +221,9 @@ class GatheredOutput:
         word = ctypes.c_uint32(0)
         stream = torch.cuda.current_stream(self.full.device).cuda_stream
         status = _abi().b200_device_status_read(ctypes.byref(word), ctypes.c_void_p(stream))
-        if status != 0 or word.value != 0:
+        if word.value == ATTENTION_OVERLAP:   # the read took it away from whoever it concerns
+            warnings.warn("attention_prompt was given offsets of sequences that overlap and returned zeros", RuntimeWarning, stacklevel=2)
+        elif status != 0 or word.value != 0:
             what = "a peer never reached the barrier" if word.value & WAIT_PEER_BARRIER else "a device-side wait gave up"
             raise RuntimeError(f"{what} (status {status}, wait sites {word.value:#x})")
 

@@ -1,7 +1,10 @@
 """What the C ABI of the serving operators accepts at its edges; no call here touches a device."""
 import ctypes
+import warnings
+from types import SimpleNamespace
 
 import pytest
+import torch
 
 from test_serving_cpu import INVALID_ARGUMENT, INVALID_PROBLEM, lib, prompt, shared  # noqa: F401  (lib: fixture)
 
@@ -32,3 +35,28 @@ def test_work_without_end_is_refused(lib, dtype):  # noqa: F811
     p = shared(dtype=dtype, batch=most, prefix=most, room=most, heads=60000, kv_heads=60000)
     assert lib.b200_attention_shared_workspace_bytes(ctypes.byref(p)) == 0
     assert lib.b200_attention_shared(ctypes.byref(p), None, 0, None) == INVALID_PROBLEM
+
+
+@pytest.mark.parametrize("word,status,outcome", [(0, 0, None), (1 << 12, 4, RuntimeWarning), (1 << 8, 6, "never reached the barrier"),
+                                                 (1 << 11, 6, "wait gave up"), (1 << 12 | 1 << 8, 6, "never reached the barrier"), (0, 5, "wait gave up")])
+def test_a_gather_is_not_blamed_for_refused_offsets(monkeypatch, word, status, outcome):
+    from cuda_ai_kernels import sharded
+
+    def read(out, stream):
+        ctypes.cast(out, ctypes.POINTER(ctypes.c_uint32))[0] = word
+        return status
+
+    monkeypatch.setattr(sharded, "_abi", lambda: SimpleNamespace(b200_device_status_read=read))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: SimpleNamespace(cuda_stream=0))
+    gathered = sharded.GatheredOutput.__new__(sharded.GatheredOutput)
+    gathered.full = torch.zeros(1)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        if outcome is None:
+            gathered.check()
+        elif outcome is RuntimeWarning:
+            with pytest.warns(RuntimeWarning, match="overlap"):
+                gathered.check()
+        else:
+            with pytest.raises(RuntimeError, match=outcome):
+                gathered.check()
